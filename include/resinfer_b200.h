@@ -301,6 +301,37 @@ int ri_resattn_get_pv_format(void);
 int64_t ri_resattn_workspace_bytes(int batch, int num_q_heads, int head_dim, int splits);
 int64_t ri_resattn_counter_bytes(int batch, int num_q_heads);
 
+/* Quantises K and V rows into a paged NVFP4 cache as they are produced, the step that the reference leaves to the
+ * serving engine's own cache write (quant/vllm_integration/attn/backend.py: stock do_kv_cache_update).
+ * Token t (of num_tokens) goes to slot slots[t] = page * page_size + offset; a negative slot, or one beyond the pool,
+ * is padding and leaves the cache alone.  The slots of one call must differ: of a slot named twice every 16-value
+ * block holds one of the tokens' codes and one of their scales.  k, v: bf16 or fp16, element (t, h, i) at
+ * t * token_stride + h * head_stride + i (strides in elements, any alignment; 16-byte aligned rows are faster).
+ * slots: int32 or int64 (slot_bits 32 / 64).  The pool is ri_resattn_decode_strided's (strides in bytes, 0 = dense);
+ * head_dim here is any multiple of 16.  A block of 16 values with largest magnitude a is held as
+ *     s = e4m3((1/g) (a / 6)), code = e2m1(x (1/g) / s), 0 where s = 0;  value = code * s * g
+ * with the rounding steps of ri_nvfp4_quant_mext for global scale 1/g (same bytes).  Values beyond 6 * 448 * g
+ * saturate, infinities among them; a NaN takes the block's largest positive code and does not count for a. */
+int ri_kv_write_nvfp4(const void* k, const void* v, int dtype, int64_t k_token_stride, int64_t k_head_stride,
+                      int64_t v_token_stride, int64_t v_head_stride, const void* slots, int slot_bits,
+                      int64_t num_tokens, uint8_t* k_data, uint8_t* k_sf, uint8_t* v_data, uint8_t* v_sf,
+                      int64_t num_pages, int64_t code_page_stride, int64_t sf_page_stride, int num_kv_heads,
+                      int head_dim, int page_size, float k_global_scale, float v_global_scale, void* stream);
+
+/* Reads held values back: k_out, v_out [num_tokens, Hkv, D] contiguous (bf16, fp16 or fp32), value = code * s * g.
+ * The tokens are named in one of two ways:
+ *   slots != NULL         one slot per row, as above; rows of negative (or out-of-range) slots become zero
+ *   block_tables != NULL  the sequences of a batch end to end: row cu_seqlens[b] + i is token i of sequence b, found
+ *                         through block_tables [batch, bt_stride] (int32, bt_cols valid columns).  Rows from
+ *                         cu_seqlens[batch] on are left as they were, or become zero with zero_tail != 0; tokens whose
+ *                         table entry is missing (negative, beyond the pool or beyond bt_cols) become zero. */
+int ri_kv_read_nvfp4(const uint8_t* k_data, const uint8_t* k_sf, const uint8_t* v_data, const uint8_t* v_sf,
+                     int64_t num_pages, int64_t code_page_stride, int64_t sf_page_stride, int num_kv_heads,
+                     int head_dim, int page_size, const void* slots, int slot_bits, const int32_t* block_tables,
+                     int64_t bt_stride, int64_t bt_cols, const int32_t* cu_seqlens, int batch, int64_t num_tokens,
+                     float k_global_scale, float v_global_scale, void* k_out, void* v_out, int out_dtype,
+                     int zero_tail, void* stream);
+
 /* Test helper: out[i] = rcp.approx.ftz.f32(in[i]) on the device (the quantisers' reciprocal). */
 int ri_rcp_approx(const float* in, float* out, int n, void* stream);
 

@@ -254,3 +254,39 @@ def run_paged_fp4_decode_qmul4_tmem_nvfp4(q: torch.Tensor, pool: NvFp4PagedKVPoo
                        float(value_scale), out, splits=splits, max_kv_len=int(max_seq_len or 0),
                        out_global_scale=gsi, out_block_scale=output_block_scale)
     return out, output_block_scale
+
+
+def _check_pool(pool: NvFp4PagedKVPool) -> None:
+    want = (pool.num_kv_heads, pool.page_size, pool.head_dim // 2)
+    if tuple(pool.k_data.shape[1:]) != want:
+        raise ValueError(f"pool.k_data must be [pages, {want[0]}, {want[1]}, {want[2]}], got {tuple(pool.k_data.shape)}")
+
+
+def write_paged_kv(key: torch.Tensor, value: torch.Tensor, pool: NvFp4PagedKVPool, slot_mapping: torch.Tensor) -> None:
+    """Quantise this step's keys and values into the pool, the write that precedes ``run_paged_fp4_decode_*``.
+
+    ``key``, ``value``: bf16 or fp16 [tokens, Hkv, D] (slices of the fused projection are taken as they are);
+    ``slot_mapping``: int32 or int64, ``page index * page_size + offset`` of every token, negative for padding; it may be
+    shorter than the rows.  Slots must be distinct.  Held with the pool's global scales; values beyond
+    ``6 * 448 * global scale`` saturate."""
+    _check_pool(pool)
+    ops.kv_write(key, value, pool.k_data, pool.k_sf, pool.v_data, pool.v_sf, slot_mapping, pool.k_global_scale,
+                 pool.v_global_scale)
+
+
+def read_paged_kv(pool: NvFp4PagedKVPool, slot_mapping: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16, out=None):
+    """(key, value) [tokens, Hkv, D] as the pool holds them in the given slots (bf16, fp16 or fp32); zero rows for
+    negative slots."""
+    _check_pool(pool)
+    return ops.kv_read(pool.k_data, pool.k_sf, pool.v_data, pool.v_sf, pool.k_global_scale, pool.v_global_scale,
+                       slots=slot_mapping, dtype=dtype, out=out)
+
+
+def gather_paged_kv(pool: NvFp4PagedKVPool, block_tables: torch.Tensor, cu_seqlens: torch.Tensor, num_tokens: int, *,
+                    dtype: torch.dtype = torch.bfloat16, out=None):
+    """(key, value) [num_tokens, Hkv, D] of the sequences of a batch end to end: row ``cu_seqlens[b] + i`` is token i of
+    sequence b, for attention over cached contexts in 16 bits.  Rows behind the last sequence are left alone in a
+    caller's ``out`` and zero otherwise."""
+    _check_pool(pool)
+    return ops.kv_read(pool.k_data, pool.k_sf, pool.v_data, pool.v_sf, pool.k_global_scale, pool.v_global_scale,
+                       block_tables=block_tables, cu_seqlens=cu_seqlens, num_tokens=num_tokens, dtype=dtype, out=out)

@@ -277,6 +277,101 @@ def resattn_decode(q: torch.Tensor, k_data: torch.Tensor, k_sf: torch.Tensor, v_
     return out
 
 
+def _kv_pool_args(k_data: torch.Tensor, k_sf: torch.Tensor, v_data: torch.Tensor, v_sf: torch.Tensor):
+    """(num_pages, code stride, scale stride, Hkv, D, page_size) of a paged NVFP4 pool, shapes and devices checked."""
+    if k_data.dim() != 4 or v_data.shape != k_data.shape or k_sf.dim() != 4 or v_sf.shape != k_sf.shape:
+        raise ValueError(f"a paged NVFP4 pool is codes [pages, Hkv, page, D/2] and scales [pages, Hkv, page, D/16] for K and V, got "
+                         f"{tuple(k_data.shape)} / {tuple(k_sf.shape)} and {tuple(v_data.shape)} / {tuple(v_sf.shape)}")
+    pages, hkv, page, half = k_data.shape
+    if half % 8 or tuple(k_sf.shape) != (pages, hkv, page, half // 8):
+        raise ValueError(f"block scales of codes {tuple(k_data.shape)} must be [pages, Hkv, page, D/16] with D a multiple of 16, got {tuple(k_sf.shape)}")
+    if not k_data.is_cuda or not (k_data.device == k_sf.device == v_data.device == v_sf.device):
+        raise ValueError("the four tensors of a pool must be on one CUDA device")
+    code_stride, sf_stride = kv_page_strides(k_data, k_sf, v_data, v_sf)
+    return pages, code_stride, sf_stride, hkv, half * 2, page
+
+
+def _check_slots(slots: torch.Tensor, device) -> int:
+    if slots.dim() != 1 or slots.dtype not in (torch.int32, torch.int64) or slots.device != device or not slots.is_contiguous():
+        raise ValueError(f"slots must be contiguous 1-D int32 or int64 on {device}, got {slots.dtype} {tuple(slots.shape)} on {slots.device}")
+    return 64 if slots.dtype == torch.int64 else 32
+
+
+def kv_write(k: torch.Tensor, v: torch.Tensor, k_data: torch.Tensor, k_sf: torch.Tensor, v_data: torch.Tensor,
+             v_sf: torch.Tensor, slots: torch.Tensor, k_global_scale: float, v_global_scale: float) -> None:
+    """Quantise K and V rows into a paged NVFP4 cache (``ri_kv_write_nvfp4``).
+
+    k, v: bf16 or fp16 [T, Hkv, D], unit stride along D, any other strides (slices of a fused projection).  ``slots``:
+    int32 / int64, one per token: ``page index * page_size + offset``; negative = padding.  Fewer slots than rows: the
+    rows behind the last slot are not written.  Slots must be distinct.  Pool tensors as for ``resattn_decode``, head_dim any
+    multiple of 16.  The bytes are those of the NVFP4 quantisers with global scale ``1 / *_global_scale``."""
+    pages, code_stride, sf_stride, hkv, d, page = _kv_pool_args(k_data, k_sf, v_data, v_sf)
+    dev = k_data.device
+    bits = _check_slots(slots, dev)
+    n = slots.shape[0]
+    for name, x in (("k", k), ("v", v)):
+        if (x.dim() != 3 or x.shape[0] < n or x.shape[1] != hkv or x.shape[2] != d or x.dtype != k.dtype or x.device != dev
+                or x.dtype not in (torch.bfloat16, torch.float16) or x.stride(2) != 1):
+            raise ValueError(f"{name} must be bf16 or fp16 [>= {n}, {hkv}, {d}] on {dev} with unit stride along the head dimension, got "
+                             f"{x.dtype} {tuple(x.shape)} strides {tuple(x.stride())} on {x.device}")
+    with _on_device(dev):
+        st = _cabi.load().ri_kv_write_nvfp4(
+            k.data_ptr(), v.data_ptr(), _cabi.torch_dtype_code(k.dtype), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+            slots.data_ptr(), bits, n, k_data.data_ptr(), k_sf.data_ptr(), v_data.data_ptr(), v_sf.data_ptr(), pages,
+            code_stride, sf_stride, hkv, d, page, k_global_scale, v_global_scale, _cabi.current_stream(dev))
+    _cabi.check(st, "kv_write")
+
+
+def kv_read(k_data: torch.Tensor, k_sf: torch.Tensor, v_data: torch.Tensor, v_sf: torch.Tensor, k_global_scale: float,
+            v_global_scale: float, *, slots: torch.Tensor | None = None, block_tables: torch.Tensor | None = None,
+            cu_seqlens: torch.Tensor | None = None, num_tokens: int | None = None, dtype: torch.dtype = torch.bfloat16,
+            out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Held values of a paged NVFP4 cache as dense K and V rows [tokens, Hkv, D] (``ri_kv_read_nvfp4``): bf16, fp16 or fp32.
+
+    Either ``slots`` (one per row; rows of negative slots are zero), or ``block_tables`` int32 [B, max pages] with
+    ``cu_seqlens`` int32 [B + 1] and ``num_tokens`` rows: the sequences of the batch end to end.  Rows behind the last
+    sequence stay as they are in a caller's ``out`` and are zero otherwise; tokens without a table entry are zero."""
+    pages, code_stride, sf_stride, hkv, d, page = _kv_pool_args(k_data, k_sf, v_data, v_sf)
+    dev = k_data.device
+    bits, bt_stride, bt_cols, batch = 64, 0, 0, 0
+    if slots is not None:
+        if block_tables is not None or cu_seqlens is not None:
+            raise ValueError("give slots, or block_tables with cu_seqlens, not both")
+        bits = _check_slots(slots, dev)
+        if num_tokens not in (None, slots.shape[0]):
+            raise ValueError(f"num_tokens {num_tokens} does not match {slots.shape[0]} slots")
+        n = slots.shape[0]
+    else:
+        if block_tables is None or cu_seqlens is None or num_tokens is None:
+            raise ValueError("give slots, or block_tables with cu_seqlens and num_tokens")
+        batch = block_tables.shape[0] if block_tables.dim() == 2 else 0
+        if (batch < 1 or block_tables.dtype != torch.int32 or block_tables.device != dev or block_tables.shape[1] < 1
+                or block_tables.stride(1) != 1):
+            raise ValueError(f"block_tables must be int32 [batch, max_pages_per_seq] on {dev} with unit column stride")
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.device != dev or tuple(cu_seqlens.shape) != (batch + 1,) or not cu_seqlens.is_contiguous():
+            raise ValueError(f"cu_seqlens must be contiguous int32 [{batch + 1}] on {dev}")
+        n, bt_stride, bt_cols = int(num_tokens), block_tables.stride(0), block_tables.shape[1]
+        if n < 0:
+            raise ValueError(f"num_tokens must not be negative, got {n}")
+    zero_tail = out is None
+    if out is None:
+        k_out = torch.empty(n, hkv, d, dtype=dtype, device=dev)
+        v_out = torch.empty(n, hkv, d, dtype=dtype, device=dev)
+    else:
+        k_out, v_out = out
+        for x in out:
+            if tuple(x.shape) != (n, hkv, d) or x.dtype != k_out.dtype or x.device != dev or not x.is_contiguous():
+                raise ValueError(f"out must be two contiguous [{n}, {hkv}, {d}] tensors of one type on {dev}")
+    with _on_device(dev):
+        st = _cabi.load().ri_kv_read_nvfp4(
+            k_data.data_ptr(), k_sf.data_ptr(), v_data.data_ptr(), v_sf.data_ptr(), pages, code_stride, sf_stride, hkv, d, page,
+            _cabi.ptr(slots), bits, _cabi.ptr(block_tables), bt_stride, bt_cols, _cabi.ptr(cu_seqlens), batch, n,
+            k_global_scale, v_global_scale, k_out.data_ptr(), v_out.data_ptr(),
+            _cabi.torch_dtype_code(k_out.dtype, allow_f32=True), int(zero_tail), _cabi.current_stream(dev))
+    _cabi.check(st, "kv_read")
+    return k_out, v_out
+
+
 def rcp_approx(x: torch.Tensor) -> torch.Tensor:
     """rcp.approx.ftz.f32 of a float32 CUDA tensor (test helper)."""
     lib = _cabi.load()
