@@ -301,6 +301,28 @@ int ri_resattn_get_pv_format(void);
 int64_t ri_resattn_workspace_bytes(int batch, int num_q_heads, int head_dim, int splits);
 int64_t ri_resattn_counter_bytes(int batch, int num_q_heads);
 
+/* ri_resattn_decode_strided for a batch whose sequences share their first prefix_len tokens (a system prompt, a document,
+ * the prompt of many samples): those tokens are read and multiplied once for all sequences.  The reference refuses such
+ * batches (quant/vllm_integration/attn/backend.py: "causal, non-cascade attention").  The result is that of
+ * ri_resattn_decode_strided on the same block tables (q residue on, FP16 V and P whatever ri_resattn_set_pv_format says).
+ *   block_tables [batch, bt_stride] (bt_cols valid columns) cover every sequence from its first token; prefix_table is a
+ *   row that holds the prefix's pages (usually block_tables itself, its first row).  A sequence no longer than the prefix
+ *   attends to its own seq_lens[b] tokens of it; an empty one gives zeros.  The prefix may end inside a page (sequences
+ *   then have copies of that page).
+ *   prefix_splits   pieces of the prefix (the grid of the first launch: pieces x KV heads x 128-row tiles); 0 = no such
+ *                   launch, every sequence reads all its tokens
+ *   splits          pieces of the tokens behind the prefix, per sequence
+ *   workspace       ri_resattn_shared_prefix_workspace_bytes() bytes, 16-byte aligned, contents of no matter, owned by this
+ *                   call until it has run: partials (o, l, m) of all pieces, and tickets
+ *   out             bf16 or fp32 [B, Hq, D]; score_scale > 0 */
+int ri_resattn_decode_shared_prefix(
+    const void* q_bf16, const uint8_t* k_data, const uint8_t* k_sf, const uint8_t* v_data, const uint8_t* v_sf,
+    int64_t num_pages, int64_t code_page_stride, int64_t sf_page_stride, const int32_t* block_tables, int64_t bt_stride,
+    int64_t bt_cols, const int32_t* prefix_table, const int32_t* seq_lens, int prefix_len, int batch, int num_q_heads,
+    int num_kv_heads, int head_dim, int page_size, int max_kv_len, float score_scale, float out_scale, void* out,
+    int out_dtype, int prefix_splits, int splits, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+int64_t ri_resattn_shared_prefix_workspace_bytes(int batch, int num_q_heads, int head_dim, int prefix_splits, int splits);
+
 /* Quantises K and V rows into a paged NVFP4 cache as they are produced, the step that the reference leaves to the
  * serving engine's own cache write (quant/vllm_integration/attn/backend.py: stock do_kv_cache_update).
  * Token t (of num_tokens) goes to slot slots[t] = page * page_size + offset; a negative slot, or one beyond the pool,

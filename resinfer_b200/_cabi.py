@@ -57,6 +57,9 @@ SIGNATURES = {
     "ri_peer_allreduce_state_bytes": (_i64, []),
     "ri_peer_allreduce_set_wait_ms": (None, [_i]),
     "ri_peer_allreduce_bf16": (_i, [_vp, _vp, _i, _i, _i64, _vp, _vp, _vp, _vp, _i]),
+    "ri_resattn_decode_shared_prefix": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i, _i, _i,
+                                             _i, _i, _i, _i, _f, _f, _vp, _i, _i, _i, _vp, _i64, _vp, _vp]),
+    "ri_resattn_shared_prefix_workspace_bytes": (_i64, [_i, _i, _i, _i, _i]),
     "ri_kv_write_nvfp4": (_i, [_vp, _vp, _i, _i64, _i64, _i64, _i64, _vp, _i, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
                                _i, _i, _i, _f, _f, _vp]),
     "ri_kv_read_nvfp4": (_i, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i, _i, _i, _vp, _i, _vp, _i64, _i64, _vp, _i, _i64,

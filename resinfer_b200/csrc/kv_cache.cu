@@ -79,19 +79,19 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const DenseIn in, const T
   const int unit = blockIdx.y * blockDim.x + threadIdx.x;
   const int64_t tok = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
   if (unit >= p.hkv * p.blocks || tok >= t.num_tokens) return;
-  const int64_t slot = load_slot(t, tok);
-  if (slot < 0 || slot >= p.num_slots) return;         // padding
   const int head = unit / p.blocks, blk = unit - head * p.blocks;
   const T* ks = static_cast<const T*>(in.k) + tok * in.k_token + head * in.k_head + blk * 16;
   const T* vs = static_cast<const T*>(in.v) + tok * in.v_token + head * in.v_head + blk * 16;
+  const int64_t slot = load_slot(t, tok);
   float kx[16], vx[16];
-  if constexpr (VEC) {
+  if constexpr (VEC) {                                 // loaded before the slot is looked at: one memory latency, not two
     load16(ks, kx);
     load16(vs, vx);
   } else {
     load16_any(ks, kx);
     load16_any(vs, vx);
   }
+  if (slot < 0 || slot >= p.num_slots) return;         // padding
   int64_t code, sf;
   slot_offsets(p, slot, head, blk, code, sf);
   auto store = [&](const float (&x)[16], float gs, uint8_t* codes, uint8_t* scales) {
@@ -119,10 +119,20 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
+__device__ __forceinline__ void store32(void* dst, const uint32_t (&w)[8]) {   // 32 bytes to a 16-byte aligned address
+  if ((reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+  } else {
+    static_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    static_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
 // one held block -> 16 values of the output row.  code * s is exact in FP32 (6 significant bits), the product with
 // the global scale is rounded once to FP32 and once to the output type.
 template <typename T>
-__device__ __forceinline__ void store_held16(T* dst, uint2 codes, uint8_t sf_byte, float gs, bool zero) {
+__device__ __forceinline__ void store_held16(T* dst, uint2 codes, uint8_t sf_byte, float gs) {
   float x[16];
   float lo[8], hi[8];
   e2m1x8_to_float(codes.x, lo);
@@ -130,66 +140,89 @@ __device__ __forceinline__ void store_held16(T* dst, uint2 codes, uint8_t sf_byt
   const float s = decode_e4m3(sf_byte);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    x[i] = zero ? 0.f : (lo[i] * s) * gs;
-    x[8 + i] = zero ? 0.f : (hi[i] * s) * gs;
+    x[i] = (lo[i] * s) * gs;
+    x[8 + i] = (hi[i] * s) * gs;
   }
+  uint32_t w[8];
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      reinterpret_cast<float4*>(dst)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(x[8 * h + i]);
+      store32(dst + 8 * h, w);
+    }
   } else {
-    uint32_t w[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
-    reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    store32(dst, w);
   }
 }
 
-template <typename T, bool BATCH>
+// NT tokens per thread, blockDim.y apart: their table look-ups and their loads are in flight together.
+template <typename T, bool BATCH, int NT>
 __global__ void __launch_bounds__(256) kv_read_kernel(T* __restrict__ k_out, T* __restrict__ v_out, const TokenRef t,
                                                       const PoolRef p, float k_gs, float v_gs, int zero_tail) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int unit = blockIdx.y * blockDim.x + threadIdx.x;
-  const int64_t tok = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
-  if (unit >= p.hkv * p.blocks || tok >= t.num_tokens) return;
-  int64_t slot = -1;
-  if constexpr (BATCH) {
-    if (tok >= __ldg(t.cu_seqlens + t.batch) && !zero_tail) return;   // rows behind the last sequence stay as they are
-    // last sequence that starts at or before `tok`
-    int lo = 0, hi = t.batch;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (__ldg(t.cu_seqlens + mid) <= tok) lo = mid;
-      else hi = mid;
-    }
-    const int64_t pos = tok - __ldg(t.cu_seqlens + lo);
-    if (pos >= 0 && tok < __ldg(t.cu_seqlens + lo + 1)) {
-      const int64_t col = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
-      if (col < t.bt_cols) {
-        const int64_t page = __ldg(t.block_tables + lo * t.bt_stride + col);
-        slot = page * p.page_size + (pos - col * p.page_size);        // negative for an unused table entry
-      }
-    }
-  } else {
-    slot = load_slot(t, tok);
-  }
-  const bool zero = slot < 0 || slot >= p.num_slots;
+  if (unit >= p.hkv * p.blocks) return;
   const int head = unit / p.blocks, blk = unit - head * p.blocks;
-  uint2 kc = make_uint2(0, 0), vc = kc;
-  uint8_t ksf = 0, vsf = 0;
-  if (!zero) {
-    int64_t code, sf;
-    slot_offsets(p, slot, head, blk, code, sf);
-    kc = __ldg(reinterpret_cast<const uint2*>(p.k_data + code));
-    vc = __ldg(reinterpret_cast<const uint2*>(p.v_data + code));
-    ksf = __ldg(p.k_sf + sf);
-    vsf = __ldg(p.v_sf + sf);
+  const int64_t tok0 = int64_t(blockIdx.x) * (blockDim.y * NT) + threadIdx.y;
+  int64_t slot[NT];
+  bool write[NT];
+  int seq = 0;                                                        // sequence of this thread's last token
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int64_t tok = tok0 + j * int(blockDim.y);
+    write[j] = tok < t.num_tokens;
+    slot[j] = -1;
+    if (!write[j]) continue;
+    if constexpr (BATCH) {
+      // the sequence of `tok`: the next one's start is beyond it.  Usually the last token's; else searched
+      if (j == 0 || tok >= __ldg(t.cu_seqlens + seq + 1)) {
+        int hi = t.batch;
+        while (hi - seq > 1) {
+          const int mid = (seq + hi) >> 1;
+          if (__ldg(t.cu_seqlens + mid) <= tok) seq = mid;
+          else hi = mid;
+        }
+      }
+      const int64_t pos = tok - __ldg(t.cu_seqlens + seq);
+      if (pos >= 0 && tok < __ldg(t.cu_seqlens + seq + 1)) {
+        const int64_t col = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
+        if (col < t.bt_cols) {
+          const int64_t page = __ldg(t.block_tables + seq * t.bt_stride + col);
+          slot[j] = page * p.page_size + (pos - col * p.page_size);   // negative for an unused table entry
+        }
+      } else if (tok >= __ldg(t.cu_seqlens + t.batch) && !zero_tail) {
+        write[j] = false;                                             // rows behind the last sequence stay as they are
+      }
+    } else {
+      slot[j] = load_slot(t, tok);
+    }
   }
-  const int64_t dst = (tok * p.hkv * p.blocks + unit) * 16;
-  store_held16(k_out + dst, kc, ksf, k_gs, zero);
-  store_held16(v_out + dst, vc, vsf, v_gs, zero);
+  uint2 kc[NT], vc[NT];
+  uint8_t ksf[NT], vsf[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    kc[j] = vc[j] = make_uint2(0, 0);                                 // no slot: code 0 times scale 0
+    ksf[j] = vsf[j] = 0;
+    if (slot[j] >= 0 && slot[j] < p.num_slots) {
+      int64_t code, sf;
+      slot_offsets(p, slot[j], head, blk, code, sf);
+      kc[j] = __ldg(reinterpret_cast<const uint2*>(p.k_data + code));
+      vc[j] = __ldg(reinterpret_cast<const uint2*>(p.v_data + code));
+      ksf[j] = __ldg(p.k_sf + sf);
+      vsf[j] = __ldg(p.v_sf + sf);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    if (!write[j]) continue;
+    const int64_t dst = ((tok0 + j * int(blockDim.y)) * (p.hkv * p.blocks) + unit) * 16;
+    store_held16(k_out + dst, kc[j], ksf[j], k_gs);
+    store_held16(v_out + dst, vc[j], vsf[j], v_gs);
+  }
 }
 
 int check_pool(PoolRef* p, const uint8_t* k_data, const uint8_t* k_sf, const uint8_t* v_data, const uint8_t* v_sf,
@@ -229,11 +262,12 @@ int check_scale(float g, const char* name) {
 }
 
 // threads of a CTA: x over a token's blocks, y over tokens
-void geometry(int64_t tokens, int units, cudaLaunchConfig_t* cfg) {
+void geometry(int64_t tokens, int units, int per_thread, cudaLaunchConfig_t* cfg) {
   const int tx = units < 256 ? units : 256;
   const int ty = 256 / tx;
+  const int64_t per_cta = int64_t(ty) * per_thread;
   cfg->blockDim = dim3(tx, ty);
-  cfg->gridDim = dim3((unsigned)((tokens + ty - 1) / ty), (unsigned)((units + tx - 1) / tx));
+  cfg->gridDim = dim3((unsigned)((tokens + per_cta - 1) / per_cta), (unsigned)((units + tx - 1) / tx));
 }
 
 }  // namespace
@@ -265,7 +299,7 @@ extern "C" int ri_kv_write_nvfp4(const void* k, const void* v, int dtype, int64_
   const bool vec = (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0) &&
                    ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) == 0;
   cudaLaunchConfig_t cfg{};
-  geometry(num_tokens, num_kv_heads * (head_dim / 16), &cfg);
+  geometry(num_tokens, num_kv_heads * (head_dim / 16), 1, &cfg);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -306,7 +340,9 @@ extern "C" int ri_kv_read_nvfp4(const uint8_t* k_data, const uint8_t* k_sf, cons
   t.slots = slots; t.slots64 = slot_bits == 64; t.num_tokens = num_tokens;
   t.block_tables = block_tables; t.bt_stride = bt_stride; t.bt_cols = bt_cols; t.cu_seqlens = cu_seqlens; t.batch = batch;
   cudaLaunchConfig_t cfg{};
-  geometry(num_tokens, num_kv_heads * (head_dim / 16), &cfg);
+  const int units = num_kv_heads * (head_dim / 16);
+  const bool wide = num_tokens * units >= int64_t(di.sm_count) * 2048 * 4;
+  geometry(num_tokens, units, wide ? 4 : 1, &cfg);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -317,9 +353,11 @@ extern "C" int ri_kv_read_nvfp4(const uint8_t* k_data, const uint8_t* k_sf, cons
     using T = std::remove_pointer_t<decltype(type)>;
     T* ko = static_cast<T*>(k_out);
     T* vo = static_cast<T*>(v_out);
-    if (by_batch)
-      return cuda_status(cudaLaunchKernelEx(&cfg, kv_read_kernel<T, true>, ko, vo, t, p, k_global_scale, v_global_scale, zero_tail), "KV cache read launch");
-    return cuda_status(cudaLaunchKernelEx(&cfg, kv_read_kernel<T, false>, ko, vo, t, p, k_global_scale, v_global_scale, zero_tail), "KV cache read launch");
+    auto launch = [&](auto kernel) {
+      return cuda_status(cudaLaunchKernelEx(&cfg, kernel, ko, vo, t, p, k_global_scale, v_global_scale, zero_tail), "KV cache read launch");
+    };
+    if (by_batch) return wide ? launch(kv_read_kernel<T, true, 4>) : launch(kv_read_kernel<T, true, 1>);
+    return wide ? launch(kv_read_kernel<T, false, 4>) : launch(kv_read_kernel<T, false, 1>);
   };
   if (out_dtype == RI_DTYPE_BF16) return go(static_cast<__nv_bfloat16*>(nullptr));
   if (out_dtype == RI_DTYPE_FP16) return go(static_cast<__half*>(nullptr));

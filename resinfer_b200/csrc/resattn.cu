@@ -11,6 +11,8 @@
 //
 // Stands in for the reference's CuTeDSL decode kernel and its reducers (ShawRong/ResInfer
 // csrc/resattn/kernel_paged_decode.py:722-2433, 2729-2861).
+#include <math.h>
+
 #include "common.cuh"
 #include "resinfer_b200.h"
 #include "tc05.cuh"
@@ -47,6 +49,12 @@ struct AttnParams {
   int sm_count;                            // host side only: SMs of the device
   int cluster_merge;                       // the splits of a (sequence, KV head) are one cluster and merge through its shared memory
   int32_t* status;
+  // shared-prefix decode only
+  int prefix_len, prefix_splits;           // tokens of the prefix, pieces its launch cuts it into (0: no such launch)
+  int steps_per_split;                     // 64-token steps of a piece
+  int max_tokens;                          // what a block table row can hold
+  int kv_begin;                            // first token of the second launch (the prefix's length, or 0)
+  const int32_t* prefix_table;             // page table row that holds the prefix
 };
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
@@ -90,6 +98,7 @@ __device__ __forceinline__ uint32_t swz_off(int row, int byte) {
 }
 
 #include "resattn_pv.cuh"
+#include "resattn_prefix.cuh"
 }  // namespace tcattn
 
 
@@ -259,4 +268,101 @@ extern "C" int ri_resattn_decode(const void* q_bf16, const uint8_t* k_data, cons
                                    out_scale, out, out_dtype, q_pack, q_pack_bytes, q_sf, q_sf_bytes, out_global_scale,
                                    out_block_scale, out_block_scale_bytes, splits, RI_ATTN_REDUCER_TICKET, workspace,
                                    workspace_bytes, q_residue, status, stream);
+}
+
+extern "C" int64_t ri_resattn_shared_prefix_workspace_bytes(int batch, int num_q_heads, int head_dim, int prefix_splits,
+                                                            int splits) {
+  if (batch < 0 || num_q_heads < 1 || head_dim < 1 || prefix_splits < 0 || splits < 1) return -1;
+  const int64_t rows = int64_t(prefix_splits + splits) * batch * num_q_heads;
+  return ri_resattn_counter_bytes(batch, num_q_heads) + rows * head_dim * 4 + 2 * rows * 4;
+}
+
+extern "C" int ri_resattn_decode_shared_prefix(
+    const void* q_bf16, const uint8_t* k_data, const uint8_t* k_sf, const uint8_t* v_data, const uint8_t* v_sf,
+    int64_t num_pages, int64_t code_page_stride, int64_t sf_page_stride, const int32_t* block_tables, int64_t bt_stride,
+    int64_t bt_cols, const int32_t* prefix_table, const int32_t* seq_lens, int prefix_len, int batch, int num_q_heads,
+    int num_kv_heads, int head_dim, int page_size, int max_kv_len, float score_scale, float out_scale, void* out,
+    int out_dtype, int prefix_splits, int splits, void* workspace, int64_t workspace_bytes, int32_t* status,
+    void* stream) {
+  RI_CHECK_ARG(head_dim == 128 || head_dim == 256, "ResAttn supports head_dim=128 or 256");
+  RI_CHECK_ARG(out_dtype == RI_DTYPE_BF16 || out_dtype == RI_DTYPE_F32, "output must be bf16 or fp32");
+  RI_CHECK_ARG(num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0, "H_q=%d must be divisible by H_kv=%d",
+               num_q_heads, num_kv_heads);
+  const int group = num_q_heads / num_kv_heads;
+  RI_CHECK_ARG(group == 4 || group == 6 || group == 8,
+               "decode residue Q8/Q16 supports logical GQA ratios (4, 6, 8), got %d", group);
+  RI_CHECK_ARG(page_size >= 16 && page_size % 16 == 0, "page size must be a multiple of 16, got %d", page_size);
+  RI_CHECK_ARG(batch >= 0 && batch <= 65535 && num_pages > 0 && bt_cols >= 1 && bt_stride >= 0 && num_kv_heads <= 65535,
+               "bad batch / page pool / block table");
+  const int64_t cap = bt_cols * page_size;
+  RI_CHECK_ARG(cap < (int64_t(1) << 31) - 256, "a block table of %lld tokens is too long", (long long)cap);
+  RI_CHECK_ARG(prefix_len >= 0 && prefix_len <= cap, "the prefix (%d tokens) must lie within the block table (%lld)", prefix_len,
+               (long long)cap);
+  RI_CHECK_ARG(max_kv_len >= 0, "max_kv_len must be non-negative");
+  RI_CHECK_ARG(score_scale > 0.f && isfinite(score_scale) && isfinite(out_scale), "score_scale must be positive and finite, out_scale finite");
+  RI_CHECK_ARG(splits >= 1 && splits <= 256 && prefix_splits >= 0 && prefix_splits <= 256, "splits must be in [1, 256], prefix splits in [0, 256]");
+  const int64_t row_tiles = (int64_t(batch) * group + 127) / 128;
+  RI_CHECK_ARG(row_tiles * num_kv_heads <= 65535, "%d sequences of %d heads are too many rows", batch, num_q_heads);
+  {
+    const int64_t page_rows = int64_t(num_kv_heads) * page_size;
+    if (code_page_stride == 0) code_page_stride = page_rows * (head_dim / 2);
+    if (sf_page_stride == 0) sf_page_stride = page_rows * (head_dim / 16);
+    RI_CHECK_ARG(code_page_stride >= page_rows * (head_dim / 2) && sf_page_stride >= page_rows * (head_dim / 16) &&
+                     code_page_stride % 16 == 0 && sf_page_stride % 16 == 0,
+                 "page strides (%lld, %lld bytes) must be multiples of 16 and hold a page's %lld rows",
+                 (long long)code_page_stride, (long long)sf_page_stride, (long long)page_rows);
+  }
+  RI_CHECK_ARG(batch == 0 || (q_bf16 && k_data && k_sf && v_data && v_sf && block_tables && seq_lens && out && prefix_table),
+               "tensors must not be null");
+  RI_CHECK_ARG(((reinterpret_cast<uintptr_t>(k_data) | reinterpret_cast<uintptr_t>(v_data) | reinterpret_cast<uintptr_t>(k_sf) |
+                 reinterpret_cast<uintptr_t>(v_sf) | reinterpret_cast<uintptr_t>(q_bf16) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
+               "q, out and the KV pool must be 16-byte aligned");
+  const int64_t need = ri_resattn_shared_prefix_workspace_bytes(batch, num_q_heads, head_dim, prefix_splits, splits);
+  RI_CHECK_ARG(batch == 0 || (workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
+               "%d + %d splits need a 16-byte aligned workspace of %lld bytes, got %lld", prefix_splits, splits, (long long)need,
+               (long long)workspace_bytes);
+  if (batch == 0) return RI_OK;
+  DeviceInfo di;
+  int s = device_info(&di);
+  if (s) return s;
+  AttnParams p{};
+  p.q = static_cast<const __nv_bfloat16*>(q_bf16);
+  p.k_data = k_data; p.k_sf = k_sf; p.v_data = v_data; p.v_sf = v_sf;
+  p.block_tables = block_tables; p.bt_stride = bt_stride; p.seq_lens = seq_lens; p.num_pages = num_pages;
+  p.code_page_stride = code_page_stride; p.sf_page_stride = sf_page_stride;
+  p.batch = batch; p.hq = num_q_heads; p.hkv = num_kv_heads; p.group = group; p.page_size = page_size;
+  p.page_shift = -1;
+  for (int sft = 4; sft < 31; ++sft)
+    if ((1 << sft) == page_size) p.page_shift = sft;
+  p.tma_pages = (page_size % 128 == 0 && num_pages < (int64_t(1) << 31)) ? 1 : 0;
+  p.score_scale_log2 = score_scale * kLog2e;
+  p.out_scale = out_scale;
+  p.out = out;
+  p.out_f32 = out_dtype == RI_DTYPE_F32;
+  p.splits = splits; p.q_residue = 1; p.status = status; p.sm_count = di.sm_count;
+  p.prefix_len = prefix_len; p.prefix_splits = prefix_splits; p.prefix_table = prefix_table;
+  p.kv_begin = prefix_splits > 0 ? prefix_len : 0;
+  p.max_tokens = int(cap);
+  {
+    const int64_t steps = (int64_t(prefix_len) + 63) / 64;
+    p.steps_per_split = prefix_splits > 0 ? int((steps + prefix_splits - 1) / prefix_splits) : 0;
+    // tiles from the one that holds token kv_begin to the longest sequence's last one
+    const int64_t bound = max_kv_len > 0 && max_kv_len < cap ? max_kv_len : cap;
+    const int64_t tiles = (bound + 127) / 128 - p.kv_begin / 128;
+    p.tiles_per_split = int((tiles + splits - 1) / splits);
+    if (p.tiles_per_split < 1) p.tiles_per_split = 1;
+  }
+  const int64_t rows = int64_t(prefix_splits + splits) * batch * num_q_heads;
+  p.split_counter = static_cast<int*>(workspace);
+  p.o_part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ri_resattn_counter_bytes(batch, num_q_heads));
+  p.l_part = p.o_part + rows * head_dim;
+  p.m_part = p.l_part + rows;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (prefix_splits > 0) {
+    s = head_dim == 128 ? tcattn::launch_prefix<128>(p, prefix_splits, st) : tcattn::launch_prefix<256>(p, prefix_splits, st);
+    if (s) return s;
+  } else if (splits > 1) {
+    RI_CUDA(cudaMemsetAsync(workspace, 0, ri_resattn_counter_bytes(batch, num_q_heads), st));
+  }
+  return head_dim == 128 ? tcattn::launch_tail<128>(p, st) : tcattn::launch_tail<256>(p, st);
 }

@@ -20,7 +20,8 @@ import torch
 
 from ... import _cabi, ops
 from .kv_layout import PAGE_SIZE, SF_VEC, NvFp4PagedKVPool
-from .plan import select_decode_plan, static_compile_plans, validate_decode_plan  # noqa: F401
+from .plan import (select_decode_plan, select_shared_prefix_plan, static_compile_plans,  # noqa: F401
+                   validate_decode_plan)
 
 N_PAD = 128
 Qmul4ReductionWorkspace = Tuple[torch.Tensor, torch.Tensor, torch.Tensor]
@@ -290,3 +291,32 @@ def gather_paged_kv(pool: NvFp4PagedKVPool, block_tables: torch.Tensor, cu_seqle
     _check_pool(pool)
     return ops.kv_read(pool.k_data, pool.k_sf, pool.v_data, pool.v_sf, pool.k_global_scale, pool.v_global_scale,
                        block_tables=block_tables, cu_seqlens=cu_seqlens, num_tokens=num_tokens, dtype=dtype, out=out)
+
+
+def run_paged_fp4_decode_shared_prefix(q: torch.Tensor, pool: NvFp4PagedKVPool, block_tables: torch.Tensor,
+                                       seq_lens: torch.Tensor, prefix_len: int, sm_scale: float, out: torch.Tensor, *,
+                                       max_seq_len: int = 0, value_scale: float = 1.0, prefix_row: int = 0,
+                                       plan: tuple[int, int] | None = None,
+                                       workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """``run_paged_fp4_decode_qmul4_tmem`` for a batch whose sequences share their first ``prefix_len`` tokens (a system
+    prompt, a document, the prompt of many samples): the prefix is read and multiplied once for all of them.
+
+    ``block_tables`` and ``seq_lens`` are the decode's own: whole sequences, prefix included; row ``prefix_row`` must hold
+    all pages of the prefix (rows may be padding, of length 0, or end inside the prefix).  ``sm_scale`` includes the K
+    global scale, ``value_scale`` is the V global scale.  ``max_seq_len``: an upper bound of ``seq_lens`` (0: taken from the
+    device, which synchronises).  ``plan``: (pieces of the prefix, pieces of the rest), chosen here without it.  BF16
+    output; V and P in FP16."""
+    _check_pool(pool)
+    b, hq, d = q.shape
+    check_shape_supported(hq, pool.num_kv_heads, d, prediction=1)
+    if out.dtype != torch.bfloat16:
+        raise ValueError("out must be contiguous BF16 [B, H_q, D]")
+    if prefix_len < 0 or prefix_len > block_tables.shape[-1] * pool.page_size:
+        raise ValueError(f"prefix_len {prefix_len} does not lie within a block table row of {block_tables.shape[-1]} pages of {pool.page_size}")
+    max_len = max_seq_len or (int(seq_lens.max().item()) if b else 0)
+    if plan is None:
+        plan = select_shared_prefix_plan(b, pool.num_kv_heads, hq // pool.num_kv_heads, prefix_len, max_len,
+                                         _sm_count(str(q.device)), head_dim=d)
+    return ops.resattn_decode_shared_prefix(
+        q, pool.k_data, pool.k_sf, pool.v_data, pool.v_sf, block_tables, seq_lens, prefix_len, sm_scale, value_scale, out,
+        prefix_splits=plan[0], splits=plan[1], prefix_row=prefix_row, max_kv_len=max_len, workspace=workspace)

@@ -19,6 +19,7 @@ leaving every split at least a few tiles.
 """
 from __future__ import annotations
 
+import functools
 import os
 
 _REDUCERS = ("none", "kernel", "cga_sharded", "gmem_fused")
@@ -125,6 +126,23 @@ def _cluster_splits(batch: int, heads: int, length: int, sms: int) -> int:
     if tiles > _CLUSTER_MAX_TILES:
         return 0
     return min(8, sms // clusters, tiles)
+
+
+@functools.lru_cache(maxsize=4096)
+def select_shared_prefix_plan(batch, num_kv_heads, group, prefix_len, max_kv_len, sm_count, *, head_dim=128):
+    """(prefix_splits, splits) for a decode whose sequences share their first ``prefix_len`` tokens: the pieces of the
+    prefix (128 query rows of one KV head each; 0 = no launch of its own) and of the tokens behind it."""
+    _check_output_dimension(head_dim, False)
+    ctas_per_sm = 2 if head_dim == 128 else 1
+    slots = sm_count * ctas_per_sm
+    steps = -(-prefix_len // 64)
+    units = max(1, num_kv_heads * -(-(batch * group) // 128))
+    prefix_splits = 0
+    if steps:
+        piece = max(2, -(-steps // max(1, slots // units)))
+        prefix_splits = min(256, -(-steps // piece))
+    rest = max(0, max_kv_len - (prefix_len // 128 * 128 if prefix_splits else 0))
+    return prefix_splits, _select_splits(batch, num_kv_heads, rest, sm_count, ctas_per_sm=ctas_per_sm)
 
 
 def static_compile_plans(*, output_nvfp4=False, grouped_head_tile=16, residue_fold=True, head_dim=128):

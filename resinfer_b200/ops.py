@@ -277,6 +277,51 @@ def resattn_decode(q: torch.Tensor, k_data: torch.Tensor, k_sf: torch.Tensor, v_
     return out
 
 
+def resattn_decode_shared_prefix(q: torch.Tensor, k_data: torch.Tensor, k_sf: torch.Tensor, v_data: torch.Tensor,
+                                 v_sf: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, prefix_len: int,
+                                 score_scale: float, out_scale: float, out: torch.Tensor, *, prefix_splits: int, splits: int,
+                                 prefix_row: int = 0, max_kv_len: int = 0, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Decode attention for a batch whose sequences share their first ``prefix_len`` tokens
+    (``ri_resattn_decode_shared_prefix``): the result of ``resattn_decode`` on the same tables, the prefix read once.
+
+    q bf16 [B, Hq, D], out bf16 or fp32 [B, Hq, D], both contiguous; ``block_tables`` int32 [B, max pages] cover every sequence
+    from its first token and row ``prefix_row`` holds all pages of the prefix; ``seq_lens`` int32 [B] are whole lengths.
+    ``prefix_splits`` / ``splits``: pieces of the prefix (0: no launch for it) and of the tokens behind it, see
+    ``nvfp4.cute_attn.plan.select_shared_prefix_plan``.  ``workspace``: a uint8 buffer of
+    ``ri_resattn_shared_prefix_workspace_bytes``; without one it comes from the caching allocator on the current stream, so
+    calls on different streams, and graphs that hold them, do not share it."""
+    lib = _cabi.load()
+    pages, code_stride, sf_stride, hkv, d, page = _kv_pool_args(k_data, k_sf, v_data, v_sf)
+    dev = q.device
+    b, hq, dq = q.shape
+    if (q.dtype != torch.bfloat16 or not q.is_contiguous() or dq != d or dev != k_data.device):
+        raise ValueError(f"q must be contiguous BF16 [B, H_q, {d}] on {k_data.device}")
+    if out.shape != q.shape or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {tuple(q.shape)} on {dev}")
+    if (block_tables.dtype != torch.int32 or block_tables.device != dev or block_tables.dim() != 2 or block_tables.shape[0] != b
+            or block_tables.shape[1] < 1 or block_tables.stride(1) != 1):
+        raise ValueError("block_tables must be int32 [batch, max_pages_per_seq] on the Q device with unit column stride")
+    if seq_lens.dtype != torch.int32 or seq_lens.device != dev or tuple(seq_lens.shape) != (b,) or not seq_lens.is_contiguous():
+        raise ValueError("seq_lens must be contiguous int32 [batch] on the Q device")
+    if b and not 0 <= prefix_row < b:
+        raise ValueError(f"prefix_row {prefix_row} is not a row of the block table ({b})")
+    with _on_device(dev):
+        need = lib.ri_resattn_shared_prefix_workspace_bytes(b, hq, d, prefix_splits, splits)
+        if workspace is None:
+            workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        elif workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be contiguous uint8 on {dev}")
+        bt = block_tables.data_ptr()
+        st = lib.ri_resattn_decode_shared_prefix(
+            q.data_ptr(), k_data.data_ptr(), k_sf.data_ptr(), v_data.data_ptr(), v_sf.data_ptr(), pages, code_stride, sf_stride,
+            bt, block_tables.stride(0), block_tables.shape[1], bt + 4 * prefix_row * block_tables.stride(0),
+            seq_lens.data_ptr(), prefix_len, b, hq, hkv, d, page, max_kv_len, score_scale, out_scale, out.data_ptr(),
+            _cabi.torch_dtype_code(out.dtype, allow_f32=True), prefix_splits, splits, workspace.data_ptr(), workspace.numel(),
+            status_word(dev).data_ptr(), _cabi.current_stream(dev))
+    _cabi.check(st, "resattn_decode_shared_prefix")
+    return out
+
+
 def _kv_pool_args(k_data: torch.Tensor, k_sf: torch.Tensor, v_data: torch.Tensor, v_sf: torch.Tensor):
     """(num_pages, code stride, scale stride, Hkv, D, page_size) of a paged NVFP4 pool, shapes and devices checked."""
     if k_data.dim() != 4 or v_data.shape != k_data.shape or k_sf.dim() != 4 or v_sf.shape != k_sf.shape:
