@@ -72,11 +72,34 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// one lane polls (bounded), the warp takes its decision
+// the whole warp waits (bounded) and takes one decision
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int site) {
-  bool got = true;
-  if ((threadIdx.x & 31) == 0) got = mbar_wait(bar, parity, abort_flag, site);
-  return __all_sync(0xffffffffu, got);
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, site));
+}
+
+// two FP32 operations per instruction; a pair is (low, high) of a 64-bit register
+__device__ __forceinline__ uint64_t pair64(uint32_t lo, uint32_t hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+  return d;
+}
+__device__ __forceinline__ void unpair64(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 template <int D>
@@ -194,10 +217,11 @@ resattn_prefix_kernel(const __grid_constant__ AttnParams p) {
           for (int i = 0; i < 64; ++i)
             if (tok0 + i >= lim) s[i >> 5][i & 31] = 0xff800000u;   // -inf
         }
-        float mx = -INFINITY;
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 64; ++i) mx = fmaxf(mx, __uint_as_float(s[i >> 5][i & 31]));
-        mx *= scale;                                           // scale > 0
+        for (int i = 0; i < 64; i += 2)
+          m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(s[i >> 5][i & 31]), __uint_as_float(s[i >> 5][(i & 31) + 1]));
+        const float mx = max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]) * scale;   // scale > 0
         bool pv_seen = j == 0;
         if (__any_sync(0xffffffffu, mx > m + kLazyThreshold)) {
           const float nw = fmaxf(m, mx);
@@ -221,16 +245,23 @@ resattn_prefix_kernel(const __grid_constant__ AttnParams p) {
         }
         const float mu = m == -INFINITY ? 0.f : m;             // a row with nothing to attend to yet
         uint32_t pk[32];
-        float sum0 = 0.f, sum1 = 0.f;
+        const uint64_t scale2 = pair64(__float_as_uint(scale), __float_as_uint(scale));
+        const uint64_t mu2 = pair64(__float_as_uint(-mu), __float_as_uint(-mu));
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          const float a = fast_exp2(fmaf(__uint_as_float(s[i >> 4][(2 * i) & 31]), scale, -mu));
-          const float b = fast_exp2(fmaf(__uint_as_float(s[i >> 4][(2 * i + 1) & 31]), scale, -mu));
-          sum0 += a;
-          sum1 += b;
+          float a, b;
+          unpair64(fma2(pair64(s[i >> 4][(2 * i) & 31], s[i >> 4][(2 * i + 1) & 31]), scale2, mu2), a, b);
+          a = fast_exp2(a);
+          b = fast_exp2(b);
+          sum[i & 1] = add2(sum[i & 1], pair64(__float_as_uint(a), __float_as_uint(b)));
           pk[i] = h2_bits(__floats2half2_rn(a, b));
         }
-        l += sum0 + sum1;
+        {
+          float a, b;
+          unpair64(add2(sum[0], sum[1]), a, b);
+          l += a + b;
+        }
         if (!pv_seen && !warp_wait(smem_u32(&bar_pvdone[(j - 1) & 1]), ((j - 1) >> 1) & 1, &abort_flag, 7)) { alive = false; break; }
         tc_fence_after();
         tmem_st32(lane_base + C::kColP, pk);
@@ -331,23 +362,20 @@ resattn_prefix_kernel(const __grid_constant__ AttnParams p) {
       constexpr uint32_t kSbo = 8 * C::kRowBytes, kLayout = D == 128 ? 4u : 2u;
       const uint64_t qb_desc = desc_kmajor(smem_u32(smem), kSbo, kLayout);
       const uint64_t qr_desc = desc_kmajor(smem_u32(smem) + C::kQBytes, kSbo, kLayout);
-      bool alive = true;
-      if (elect_one()) {                                       // the query scales, once
+      if (elect_one()) {                                       // one thread: no votes, no reconvergence on the way
 #pragma unroll
-        for (int j = 0; j < 2 * C::kMma; ++j)
+        for (int j = 0; j < 2 * C::kMma; ++j)                  // the query scales, once
           tmem_cp_sf(tmem_base + C::kColSfq + 4 * j, desc_sf(smem_u32(smem) + C::kOffQsf + j * 512));
-      }
-      __syncwarp();
-      auto issue_qk = [&](int j) {
-        const int stg = j % S, sb = j & 1;
-        if (!warp_wait(smem_u32(&bar_full[stg]), (j / S) & 1, &abort_flag, 3)) { alive = false; return; }
-        if (j > 0 && !warp_wait(smem_u32(&bar_sfree), (j - 1) & 1, &abort_flag, 4)) { alive = false; return; }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // cp.async data -> tensor-core reads
-        tc_fence_after();
-        if (elect_one()) {
+        const uint32_t sfq = tmem_base + C::kColSfq;
+        auto issue_qk = [&](int j, int stg, int ph) -> bool {
+          const uint32_t sb = j & 1;
+          if (!mbar_wait(smem_u32(&bar_full[stg]), ph, &abort_flag, 3)) return false;
+          if (j > 0 && !mbar_wait(smem_u32(&bar_sfree), (j - 1) & 1, &abort_flag, 4)) return false;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // cp.async data -> tensor-core reads
+          tc_fence_after();
           const uint32_t st = smem_u32(stage0 + stg * C::kStageBytes);
           const uint64_t k_desc = desc_kmajor(st, kSbo, kLayout);
-          const uint32_t sfk = tmem_base + C::kColSfk + sb * 4 * C::kMma, sfq = tmem_base + C::kColSfq;
+          const uint32_t sfk = tmem_base + C::kColSfk + sb * 4 * C::kMma;
 #pragma unroll
           for (int i = 0; i < C::kMma; ++i) tmem_cp_sf(sfk + 4 * i, desc_sf(st + C::kStgKsf + i * 512));
 #pragma unroll
@@ -360,28 +388,26 @@ resattn_prefix_kernel(const __grid_constant__ AttnParams p) {
                            sfq + 4 * (C::kMma + i), sfk + 4 * i, 1u);
           mma_commit(smem_u32(&bar_sfull));
           mma_commit(smem_u32(&bar_empty[stg]));               // the K codes of the stage have been read
-        }
-        __syncwarp();
-      };
-      if (steps > 0) issue_qk(0);
-      for (int j = 0; j < steps && alive; ++j) {
-        if (j + 1 < steps) issue_qk(j + 1);
-        if (!alive) break;
-        const int vb = j & 1;
-        if (!warp_wait(smem_u32(&bar_vready[vb]), (j >> 1) & 1, &abort_flag, 8)) break;
-        if (!warp_wait(smem_u32(&bar_pready), j & 1, &abort_flag, 9)) break;
-        tc_fence_after();
-        if (elect_one()) {
-          // B = V: N-major, 128-byte swizzle: 64-d blocks 8 KB apart (leading offset), 8-token groups 1 KB apart
-          const uint32_t va = smem_u32(smem + C::kOffV + vb * C::kVBytes);
+          return true;
+        };
+        // B = V: N-major, 128-byte swizzle: 64-d blocks 8 KB apart (leading offset), 8-token groups 1 KB apart
+        const uint64_t v_desc = desc_full(smem_u32(smem + C::kOffV), C::kStep * 128, 1024, 2);
+        bool alive = steps > 0 && issue_qk(0, 0, 0);
+        for (int j = 0, stg = 1, ph = 0; j < steps && alive; ++j) {
+          if (j + 1 < steps && !issue_qk(j + 1, stg, ph)) break;
+          if (++stg == S) stg = 0, ph ^= 1;
+          const int vb = j & 1;
+          if (!mbar_wait(smem_u32(&bar_vready[vb]), (j >> 1) & 1, &abort_flag, 8)) break;
+          if (!mbar_wait(smem_u32(&bar_pready), j & 1, &abort_flag, 9)) break;
+          tc_fence_after();
 #pragma unroll
           for (int k16 = 0; k16 < C::kStep / 16; ++k16)
-            mma_f16_ts(tmem_base + C::kColO, tmem_base + C::kColP + 8 * k16, desc_full(va + k16 * 2048, C::kStep * 128, 1024, 2),
+            mma_f16_ts(tmem_base + C::kColO, tmem_base + C::kColP + 8 * k16, v_desc + uint64_t((vb * C::kVBytes + k16 * 2048) >> 4),
                        idesc_pv, (j > 0 || k16 > 0) ? 1u : 0u);
           mma_commit(smem_u32(&bar_pvdone[vb]));
         }
-        __syncwarp();
       }
+      __syncwarp();
     } else if (warp < 11) {
       // ============================================================ copies: warp 9 + pw, tokens 32 pw .. 32 pw + 31 of a step
       const int pw = warp - 9;
