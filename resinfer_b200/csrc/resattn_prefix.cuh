@@ -2,8 +2,8 @@
 // namespace ri::<anon>::tcattn.
 //
 // All query heads of all sequences that read one KV head are rows of one problem, R = batch x group rows against the
-// prefix's tokens, so the prefix crosses HBM once instead of once per sequence.  A CTA takes 128 rows, one KV head and a
-// range of the prefix (its split) in steps of 64 tokens:
+// prefix's tokens, so the prefix crosses HBM once instead of once per sequence.  A CTA takes NT tiles of 128 rows, one KV
+// head and a range of the prefix (its split) in steps of 64 tokens:
 //
 //   S[128 rows x 64]  = Qbase . K^T + Qres . K^T   tcgen05.mma kind::mxf4nvf4.block_scale, codes and E4M3 scales as stored
 //   P = 2^(S scale - m)                            one row per softmax thread, rounded to FP16
@@ -16,37 +16,42 @@
 //
 // Rows shorter than the prefix are masked at their own length; rows beyond the batch have length zero.
 //
-// Roles (12 warps; head_dim 128: two CTAs per SM, head_dim 256: one):
-//   0-3   softmax, thread = row (tensor-memory lane)
-//   4-7   V conversion: codes x scales -> FP16 in the 128-byte-swizzled N-major operand layout
-//   8     MMA issue; K scales shared -> tensor memory
-//   9-10  copies (cp.async, 32 tokens of a step each): pages of 16 tokens and up
-template <int D>
+// Roles:
+//   softmax     four warps per row tile, thread = row (tensor-memory lane)
+//   conversion  four warps: V codes x scales -> FP16 in the 128-byte-swizzled N-major operand layout, once for all row tiles
+//   issue       one thread per row tile: K scales shared -> tensor memory, scores of step j+1 before the P.V of step j
+//   copies      two warps of cp.async, 32 tokens of a step each: pages of 16 tokens and up
+// Every wait is bounded.  A role whose wait expires sets the abort flag, which ends all other waits at once, and runs on
+// through its loop (every address is in bounds whatever the data), so all roles meet at the end and the status word is set.
+template <int D, int NT_>
 struct PxCfg {
+  static constexpr int NT = NT_;                               // row tiles of a CTA
   static constexpr int kStep = 64;                             // tokens per step
   static constexpr int kRows = 128;
-  static constexpr int kThreads = 384;
-  static constexpr int kStages = 4;
-  static constexpr int kCtasPerSm = D == 128 ? 2 : 1;
+  static constexpr int kFirstConv = 4 * NT, kFirstIssue = kFirstConv + 4, kFirstProd = kFirstIssue + 2;
+  static constexpr int kThreads = (kFirstProd + 2) * 32;       // 12 or 16 warps: whole warpgroups
+  static constexpr int kCtasPerSm = D == 128 && NT == 1 ? 2 : 1;
+  static constexpr int kStages = kCtasPerSm == 2 ? 4 : 6;
   static constexpr int kMma = D / 64;
   static constexpr int kRowBytes = D / 2;
   static constexpr int kSfPerRow = D / 16;
   static constexpr int kDBlocks = D / 64;
-  // shared memory: Q codes (base, residue), Q scales (base, residue), V tiles, stages
+  // shared memory: per row tile Q codes (base, residue) and Q scales (base, residue); V tiles; stages
   static constexpr int kQBytes = kRows * kRowBytes;
   static constexpr int kQsfBytes = kMma * 512;
+  static constexpr int kOffQsf = 2 * kQBytes, kQTile = 2 * kQBytes + 2 * kQsfBytes;     // multiples of 1024
   static constexpr int kVBytes = kStep * D * 2;
-  static constexpr int kOffQsf = 2 * kQBytes;
-  static constexpr int kOffV = kOffQsf + 2 * kQsfBytes;        // a multiple of 1024
+  static constexpr int kOffV = NT * kQTile;
   static constexpr int kOffStage = kOffV + 2 * kVBytes;
   static constexpr int kKBytes = kStep * kRowBytes;
   static constexpr int kStgV = kKBytes, kStgKsf = 2 * kKBytes, kStgVsf = kStgKsf + kMma * 512;
   static constexpr int kStageBytes = (kStgVsf + kStep * kSfPerRow + 1023) / 1024 * 1024;
   static constexpr int kSmemBytes = kOffStage + kStages * kStageBytes + 1024;
-  // tensor memory columns
+  // tensor memory columns of a row tile: accumulator, scores, P, query scales, K scales (two sets)
   static constexpr int kColO = 0, kColS = D, kColP = D + 64, kColSfq = D + 96, kColSfk = kColSfq + 8 * kMma;
-  static constexpr int kTmemCols = D == 128 ? 256 : 512;
-  static_assert(kColSfk + 8 * kMma <= kTmemCols && kOffV % 1024 == 0, "layout");
+  static constexpr int kTileCols = D == 128 ? 256 : 512;
+  static constexpr int kTmemCols = NT * kTileCols;
+  static_assert(kColSfk + 8 * kMma <= kTileCols && kTmemCols <= 512 && kQTile % 1024 == 0, "layout");
 };
 
 // D[128 x N] += A[128 x 16, tensor memory] . B[16 x N, shared memory], FP16 operands
@@ -72,9 +77,11 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// the whole warp waits (bounded) and takes one decision
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int site) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, site));
+// A wait that returns when the phase is complete, or when the kernel has given up (see above).
+__device__ __forceinline__ void px_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int site) {
+  if (mbar_try(bar, parity)) return;
+  if (*abort_flag) return;
+  mbar_wait(bar, parity, abort_flag, site);
 }
 
 // two FP32 operations per instruction; a pair is (low, high) of a 64-bit register
@@ -102,19 +109,19 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-template <int D>
-__global__ void __launch_bounds__(PxCfg<D>::kThreads, PxCfg<D>::kCtasPerSm)
+template <int D, int NT>
+__global__ void __launch_bounds__(PxCfg<D, NT>::kThreads, PxCfg<D, NT>::kCtasPerSm)
 resattn_prefix_kernel(const __grid_constant__ AttnParams p) {
-  using C = PxCfg<D>;
+  using C = PxCfg<D, NT>;
   constexpr int S = C::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[S], bar_empty[S];
-  __shared__ __align__(8) uint64_t bar_sfull, bar_sfree, bar_pready, bar_vready[2], bar_pvdone[2];
+  __shared__ __align__(8) uint64_t bar_sfull[NT], bar_sfree[NT], bar_pready[NT], bar_pvdone[NT], bar_vready[2], bar_vfree[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = blockIdx.x, hkv = blockIdx.y % p.hkv, row0 = (blockIdx.y / p.hkv) * C::kRows;
+  const int split = blockIdx.x, hkv = blockIdx.y % p.hkv, row0 = (blockIdx.y / p.hkv) * (NT * C::kRows);
   const int G = p.group, rows = p.batch * G;
 
   // Everything this kernel reads was written before the launch in front of it ended, and the launch behind it may start
@@ -132,26 +139,30 @@ resattn_prefix_kernel(const __grid_constant__ AttnParams p) {
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(smem_u32(&bar_full[s]), 64);
-      mbar_init(smem_u32(&bar_empty[s]), 4 + 1);               // conversion warps + the commit of the scores' MMAs
+      mbar_init(smem_u32(&bar_empty[s]), 4 + NT);              // conversion warps + the commits of the scores' MMAs
     }
-    mbar_init(smem_u32(&bar_sfull), 1);
-    mbar_init(smem_u32(&bar_sfree), 4);
-    mbar_init(smem_u32(&bar_pready), 4);
+    for (int t = 0; t < NT; ++t) {
+      mbar_init(smem_u32(&bar_sfull[t]), 1);
+      mbar_init(smem_u32(&bar_sfree[t]), 4);
+      mbar_init(smem_u32(&bar_pready[t]), 4);
+      mbar_init(smem_u32(&bar_pvdone[t]), 1);
+    }
     for (int s = 0; s < 2; ++s) {
       mbar_init(smem_u32(&bar_vready[s]), 4);
-      mbar_init(smem_u32(&bar_pvdone[s]), 1);
+      mbar_init(smem_u32(&bar_vfree[s]), NT);
     }
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) {
+  if (warp == C::kFirstIssue) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(smem_u32(&tmem_slot)), "r"(C::kTmemCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   // ---------------------------------------------------------------- query prologue: NVFP4 and its NVFP4 residue
-  for (int i = threadIdx.x; i < C::kRows * C::kSfPerRow; i += blockDim.x) {
-    const int r = i / C::kSfPerRow, blk = i % C::kSfPerRow, row = row0 + r;
+  for (int i = threadIdx.x; i < NT * C::kRows * C::kSfPerRow; i += blockDim.x) {
+    const int rr = i / C::kSfPerRow, blk = i % C::kSfPerRow, row = row0 + rr;
+    const int r = rr & (C::kRows - 1);
     BlockQ bq{};
     if (row < rows) {
       const int b = row / G, g = row - b * G;
@@ -159,12 +170,13 @@ resattn_prefix_kernel(const __grid_constant__ AttnParams p) {
       load16(p.q + (int64_t(b) * p.hq + hkv * G + g) * D + blk * 16, v);
       bq = quant_mext16(v, 1.0f, 1.0f);
     }
+    uint8_t* tile = smem + (rr / C::kRows) * C::kQTile;
     const uint32_t off = swz_off<D>(r, blk * 8);
-    *reinterpret_cast<uint2*>(smem + off) = bq.base;
-    *reinterpret_cast<uint2*>(smem + C::kQBytes + off) = bq.res;
+    *reinterpret_cast<uint2*>(tile + off) = bq.base;
+    *reinterpret_cast<uint2*>(tile + C::kQBytes + off) = bq.res;
     const uint32_t so = C::kOffQsf + (blk >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (blk & 3);
-    smem[so] = bq.sf;
-    smem[so + C::kQsfBytes] = bq.sf_res;
+    tile[so] = bq.sf;
+    tile[so + C::kQsfBytes] = bq.sf_res;
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   tc_fence_before();
@@ -173,17 +185,19 @@ resattn_prefix_kernel(const __grid_constant__ AttnParams p) {
   const uint32_t tmem_base = tmem_slot;
   uint8_t* stage0 = smem + C::kOffStage;
 
-  if (warp < 4) {
+  if (warp < C::kFirstConv) {
     // ============================================================ softmax warps
-    if constexpr (D == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
-    const uint32_t lane_base = tmem_base + (uint32_t(warp * 32) << 16);
+    if constexpr (C::kCtasPerSm == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+    const int tile = warp >> 2, quarter = warp & 3;
+    const uint32_t lane_base = tmem_base + tile * C::kTileCols + (uint32_t(quarter * 32) << 16);
+    const uint32_t b_sfull = smem_u32(&bar_sfull[tile]), b_sfree = smem_u32(&bar_sfree[tile]);
+    const uint32_t b_pready = smem_u32(&bar_pready[tile]), b_pvdone = smem_u32(&bar_pvdone[tile]);
     const int row = row0 + warp * 32 + lane;
     int lim = 0;
     if (row < rows) lim = min(max(__ldg(p.seq_lens + row / G), 0), p.prefix_len);
     const int lim_min = __reduce_min_sync(0xffffffffu, lim), lim_max = __reduce_max_sync(0xffffffffu, lim);
     const float scale = p.score_scale_log2;
     float m = -INFINITY, l = 0.f;
-    bool alive = true;
     if (lim_max <= s_begin * C::kStep) {
       // none of this warp's rows reaches the split's tokens: their P is zero throughout
       uint32_t z[32];
@@ -192,17 +206,19 @@ resattn_prefix_kernel(const __grid_constant__ AttnParams p) {
       tmem_st32(lane_base + C::kColP, z);
       tmem_wait_st();
       tc_fence_before();
-      for (int j = 0; j < steps && alive; ++j) {
-        alive = warp_wait(smem_u32(&bar_sfull), j & 1, &abort_flag, 5);
-        if (alive && j > 0) alive = warp_wait(smem_u32(&bar_pvdone[(j - 1) & 1]), ((j - 1) >> 1) & 1, &abort_flag, 7);
-        if (alive && lane == 0) {
-          mbar_arrive(smem_u32(&bar_sfree));
-          mbar_arrive(smem_u32(&bar_pready));
+      for (int j = 0; j < steps; ++j) {
+        px_wait(b_sfull, j & 1, &abort_flag, 5);
+        if (j > 0) px_wait(b_pvdone, (j - 1) & 1, &abort_flag, 7);
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(b_sfree);
+          mbar_arrive(b_pready);
         }
       }
     } else {
       for (int j = 0; j < steps; ++j) {
-        if (!warp_wait(smem_u32(&bar_sfull), j & 1, &abort_flag, 5)) { alive = false; break; }
+        px_wait(b_sfull, j & 1, &abort_flag, 5);
+        __syncwarp();
         tc_fence_after();
         uint32_t s[2][32];
         tmem_ld32_async(lane_base + C::kColS, s[0]);
@@ -210,7 +226,7 @@ resattn_prefix_kernel(const __grid_constant__ AttnParams p) {
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bar_sfree));      // the next scores may overwrite S
+        if (lane == 0) mbar_arrive(b_sfree);                   // the next scores may overwrite S
         const int tok0 = (s_begin + j) * C::kStep;
         if (tok0 + C::kStep > lim_min) {
 #pragma unroll
@@ -229,7 +245,8 @@ resattn_prefix_kernel(const __grid_constant__ AttnParams p) {
           m = nw;
           l *= f;
           if (j > 0) {                                         // rescale this row's accumulator in place
-            if (!warp_wait(smem_u32(&bar_pvdone[(j - 1) & 1]), ((j - 1) >> 1) & 1, &abort_flag, 7)) { alive = false; break; }
+            px_wait(b_pvdone, (j - 1) & 1, &abort_flag, 7);
+            __syncwarp();
             pv_seen = true;
             tc_fence_after();
 #pragma unroll 1
@@ -262,21 +279,24 @@ resattn_prefix_kernel(const __grid_constant__ AttnParams p) {
           unpair64(add2(sum[0], sum[1]), a, b);
           l += a + b;
         }
-        if (!pv_seen && !warp_wait(smem_u32(&bar_pvdone[(j - 1) & 1]), ((j - 1) >> 1) & 1, &abort_flag, 7)) { alive = false; break; }
+        if (!pv_seen) {
+          px_wait(b_pvdone, (j - 1) & 1, &abort_flag, 7);
+          __syncwarp();
+        }
         tc_fence_after();
         tmem_st32(lane_base + C::kColP, pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bar_pready));
+        if (lane == 0) mbar_arrive(b_pready);
       }
     }
     // ---------------------------------------------------------------- the rows' partials
-    if (alive && steps > 0) alive = warp_wait(smem_u32(&bar_pvdone[(steps - 1) & 1]), ((steps - 1) >> 1) & 1, &abort_flag, 12);
+    if (steps > 0) px_wait(b_pvdone, (steps - 1) & 1, &abort_flag, 12);
+    __syncwarp();
     if (__any_sync(0xffffffffu, row < rows)) {                 // whole warps: the loads from tensor memory are collective
       const int b = row / G, g = row - b * G;
       const int64_t slot = (int64_t(p.splits + split) * p.batch + b) * p.hq + hkv * G + g;
-      if (!alive || steps == 0) m = -INFINITY;
       if (row < rows) {
         p.l_part[slot] = m == -INFINITY ? 0.f : l;
         p.m_part[slot] = m;
@@ -296,17 +316,16 @@ resattn_prefix_kernel(const __grid_constant__ AttnParams p) {
         tc_fence_before();
       }
     }
-  } else if (warp < 8) {
+  } else if (warp < C::kFirstIssue) {
     // ============================================================ V conversion warps
-    if constexpr (D == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    const int cw = warp - 4;
+    if constexpr (C::kCtasPerSm == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    const int cw = warp - C::kFirstConv;
+    constexpr int kPer = C::kDBlocks / 2;                      // d-blocks a thread converts
+    const int tok = 32 * (cw & 1) + lane;
     for (int j = 0, stg = 0, ph = 0; j < steps; ++j, stg = (stg + 1 == S ? 0 : stg + 1), ph ^= (stg == 0)) {
       const int vb = j & 1;
-      if (!warp_wait(smem_u32(&bar_full[stg]), ph, &abort_flag, 6)) break;
-      if (j >= 2 && !warp_wait(smem_u32(&bar_pvdone[vb]), ((j >> 1) - 1) & 1, &abort_flag, 11)) break;
+      px_wait(smem_u32(&bar_full[stg]), ph, &abort_flag, 6);
       const uint8_t* st = stage0 + stg * C::kStageBytes;
-      constexpr int kPer = C::kDBlocks / 2;                    // d-blocks a thread converts
-      const int tok = 32 * (cw & 1) + lane;
       const bool valid = (s_begin + j) * C::kStep + tok < p.prefix_len;
       uint4 c0[kPer], c1[kPer];
       uint32_t sfw[kPer];
@@ -316,14 +335,15 @@ resattn_prefix_kernel(const __grid_constant__ AttnParams p) {
         c0[u] = c1[u] = make_uint4(0, 0, 0, 0);
         sfw[u] = 0;
         if (valid) {
-          const uint8_t* row = st + C::kStgV;
-          c0[u] = *reinterpret_cast<const uint4*>(row + swz_off<D>(tok, 32 * dblk));
-          c1[u] = *reinterpret_cast<const uint4*>(row + swz_off<D>(tok, 32 * dblk + 16));
+          const uint8_t* src = st + C::kStgV;
+          c0[u] = *reinterpret_cast<const uint4*>(src + swz_off<D>(tok, 32 * dblk));
+          c1[u] = *reinterpret_cast<const uint4*>(src + swz_off<D>(tok, 32 * dblk + 16));
           sfw[u] = *reinterpret_cast<const uint32_t*>(st + C::kStgVsf + tok * C::kSfPerRow + dblk * 4);
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bar_empty[stg]));   // the codes are in registers: the stage may be refilled
+      if (j >= 2) px_wait(smem_u32(&bar_vfree[vb]), ((j >> 1) - 1) & 1, &abort_flag, 11);
 #pragma unroll
       for (int u = 0; u < kPer; ++u) {
         const int dblk = (cw >> 1) * kPer + u;
@@ -353,64 +373,67 @@ resattn_prefix_kernel(const __grid_constant__ AttnParams p) {
       if (lane == 0) mbar_arrive(smem_u32(&bar_vready[vb]));
     }
   } else {
-    if constexpr (D == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 8) {
-      // ============================================================ MMA issuer: the scores of step j+1 before the P.V of step j
+    if constexpr (C::kCtasPerSm == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp < C::kFirstIssue + NT) {
+      // ============================================================ issue: one thread per row tile
+      const int tile = warp - C::kFirstIssue;
       const uint32_t idesc_qk = (1u << 7) | (1u << 10) | (uint32_t(C::kStep >> 3) << 17) | (uint32_t(C::kRows >> 4) << 24);
       // kind::f16: FP32 accumulate, FP16 x FP16, A from tensor memory, B N-major (bit 16), N = D, M = 128
       const uint32_t idesc_pv = (1u << 4) | (1u << 16) | (uint32_t(D >> 3) << 17) | (uint32_t(C::kRows >> 4) << 24);
       constexpr uint32_t kSbo = 8 * C::kRowBytes, kLayout = D == 128 ? 4u : 2u;
-      const uint64_t qb_desc = desc_kmajor(smem_u32(smem), kSbo, kLayout);
-      const uint64_t qr_desc = desc_kmajor(smem_u32(smem) + C::kQBytes, kSbo, kLayout);
-      if (elect_one()) {                                       // one thread: no votes, no reconvergence on the way
+      if (elect_one()) {
+        const uint32_t tm = tmem_base + tile * C::kTileCols, sfq = tm + C::kColSfq;
+        const uint32_t q_addr = smem_u32(smem) + tile * C::kQTile;
+        const uint64_t qb_desc = desc_kmajor(q_addr, kSbo, kLayout), qr_desc = desc_kmajor(q_addr + C::kQBytes, kSbo, kLayout);
+        const uint32_t b_sfull = smem_u32(&bar_sfull[tile]), b_sfree = smem_u32(&bar_sfree[tile]);
+        const uint32_t b_pready = smem_u32(&bar_pready[tile]), b_pvdone = smem_u32(&bar_pvdone[tile]);
 #pragma unroll
         for (int j = 0; j < 2 * C::kMma; ++j)                  // the query scales, once
-          tmem_cp_sf(tmem_base + C::kColSfq + 4 * j, desc_sf(smem_u32(smem) + C::kOffQsf + j * 512));
-        const uint32_t sfq = tmem_base + C::kColSfq;
-        auto issue_qk = [&](int j, int stg, int ph) -> bool {
-          const uint32_t sb = j & 1;
-          if (!mbar_wait(smem_u32(&bar_full[stg]), ph, &abort_flag, 3)) return false;
-          if (j > 0 && !mbar_wait(smem_u32(&bar_sfree), (j - 1) & 1, &abort_flag, 4)) return false;
+          tmem_cp_sf(sfq + 4 * j, desc_sf(q_addr + C::kOffQsf + j * 512));
+        auto issue_qk = [&](int j, int stg, int ph) {
+          px_wait(smem_u32(&bar_full[stg]), ph, &abort_flag, 3);
+          if (j > 0) px_wait(b_sfree, (j - 1) & 1, &abort_flag, 4);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // cp.async data -> tensor-core reads
           tc_fence_after();
           const uint32_t st = smem_u32(stage0 + stg * C::kStageBytes);
           const uint64_t k_desc = desc_kmajor(st, kSbo, kLayout);
-          const uint32_t sfk = tmem_base + C::kColSfk + sb * 4 * C::kMma;
+          const uint32_t sfk = tm + C::kColSfk + (j & 1) * 4 * C::kMma;
 #pragma unroll
           for (int i = 0; i < C::kMma; ++i) tmem_cp_sf(sfk + 4 * i, desc_sf(st + C::kStgKsf + i * 512));
 #pragma unroll
           for (int i = 0; i < C::kMma; ++i)
-            mma_fp4<false>(tmem_base + C::kColS, qb_desc + uint64_t(2 * i), k_desc + uint64_t(2 * i), idesc_qk, sfq + 4 * i,
-                           sfk + 4 * i, i > 0 ? 1u : 0u);
+            mma_fp4<false>(tm + C::kColS, qb_desc + uint64_t(2 * i), k_desc + uint64_t(2 * i), idesc_qk, sfq + 4 * i, sfk + 4 * i,
+                           i > 0 ? 1u : 0u);
 #pragma unroll
           for (int i = 0; i < C::kMma; ++i)
-            mma_fp4<false>(tmem_base + C::kColS, qr_desc + uint64_t(2 * i), k_desc + uint64_t(2 * i), idesc_qk,
-                           sfq + 4 * (C::kMma + i), sfk + 4 * i, 1u);
-          mma_commit(smem_u32(&bar_sfull));
+            mma_fp4<false>(tm + C::kColS, qr_desc + uint64_t(2 * i), k_desc + uint64_t(2 * i), idesc_qk, sfq + 4 * (C::kMma + i),
+                           sfk + 4 * i, 1u);
+          mma_commit(b_sfull);
           mma_commit(smem_u32(&bar_empty[stg]));               // the K codes of the stage have been read
-          return true;
         };
         // B = V: N-major, 128-byte swizzle: 64-d blocks 8 KB apart (leading offset), 8-token groups 1 KB apart
         const uint64_t v_desc = desc_full(smem_u32(smem + C::kOffV), C::kStep * 128, 1024, 2);
-        bool alive = steps > 0 && issue_qk(0, 0, 0);
-        for (int j = 0, stg = 1, ph = 0; j < steps && alive; ++j) {
-          if (j + 1 < steps && !issue_qk(j + 1, stg, ph)) break;
+        if (steps > 0) issue_qk(0, 0, 0);
+        for (int j = 0, stg = 1, ph = 0; j < steps; ++j) {
+          if (j + 1 < steps) issue_qk(j + 1, stg, ph);
           if (++stg == S) stg = 0, ph ^= 1;
           const int vb = j & 1;
-          if (!mbar_wait(smem_u32(&bar_vready[vb]), (j >> 1) & 1, &abort_flag, 8)) break;
-          if (!mbar_wait(smem_u32(&bar_pready), j & 1, &abort_flag, 9)) break;
+          px_wait(smem_u32(&bar_vready[vb]), (j >> 1) & 1, &abort_flag, 8);
+          px_wait(b_pready, j & 1, &abort_flag, 9);
           tc_fence_after();
 #pragma unroll
           for (int k16 = 0; k16 < C::kStep / 16; ++k16)
-            mma_f16_ts(tmem_base + C::kColO, tmem_base + C::kColP + 8 * k16, v_desc + uint64_t((vb * C::kVBytes + k16 * 2048) >> 4),
-                       idesc_pv, (j > 0 || k16 > 0) ? 1u : 0u);
-          mma_commit(smem_u32(&bar_pvdone[vb]));
+            mma_f16_ts(tm + C::kColO, tm + C::kColP + 8 * k16, v_desc + uint64_t((vb * C::kVBytes + k16 * 2048) >> 4), idesc_pv,
+                       (j > 0 || k16 > 0) ? 1u : 0u);
+          mma_commit(b_pvdone);
+          mma_commit(smem_u32(&bar_vfree[vb]));
         }
+        if (steps > 0) px_wait(b_pvdone, (steps - 1) & 1, &abort_flag, 13);   // nothing of this tile is in flight any more
       }
       __syncwarp();
-    } else if (warp < 11) {
-      // ============================================================ copies: warp 9 + pw, tokens 32 pw .. 32 pw + 31 of a step
-      const int pw = warp - 9;
+    } else if (warp >= C::kFirstProd) {
+      // ============================================================ copies: warp pw, tokens 32 pw .. 32 pw + 31 of a step
+      const int pw = warp - C::kFirstProd;
       constexpr int kCpr = C::kRowBytes / 16, kRowsPerIt = 32 / kCpr, kIters = 32 / kRowsPerIt;
       const int r_lane = lane / kCpr, chn = lane % kCpr;
       auto lookup = [&](int j) -> int {                        // lanes 0 and 1: the pages of the warp's two groups of 16 tokens
@@ -434,7 +457,8 @@ resattn_prefix_kernel(const __grid_constant__ AttnParams p) {
         const int64_t code1 = pg1 * p.code_page_stride + int64_t(in1) * C::kRowBytes;
         const int64_t sf0 = pg0 * p.sf_page_stride + int64_t(in0) * C::kSfPerRow;
         const int64_t sf1 = pg1 * p.sf_page_stride + int64_t(in1) * C::kSfPerRow;
-        if (j >= S && !warp_wait(smem_u32(&bar_empty[stg]), ph ^ 1, &abort_flag, 4)) break;
+        if (j >= S) px_wait(smem_u32(&bar_empty[stg]), ph ^ 1, &abort_flag, 4);
+        __syncwarp();
         const uint32_t st = smem_u32(stage0 + stg * C::kStageBytes);
 #pragma unroll
         for (int it = 0; it < kIters; ++it) {
@@ -464,27 +488,27 @@ resattn_prefix_kernel(const __grid_constant__ AttnParams p) {
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && abort_flag != 0 && p.status) atomicExch(p.status, 1 + int(blockIdx.y) + (abort_flag << 16));
-  if (warp == 8) {
+  if (warp == C::kFirstIssue) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(C::kTmemCols) : "memory");
   }
 }
 
-template <int D>
-int launch_prefix(const AttnParams& p, int prefix_splits, cudaStream_t st) {
-  using C = PxCfg<D>;
+template <int D, int NT>
+int launch_prefix_tiles(const AttnParams& p, int prefix_splits, cudaStream_t st) {
+  using C = PxCfg<D, NT>;
   static bool attr_done[64] = {};
   int dev = 0;
   RI_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) dev = 0;
   if (!attr_done[dev]) {
-    RI_CUDA(cudaFuncSetAttribute(resattn_prefix_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
-    RI_CUDA(cudaFuncSetAttribute(resattn_prefix_kernel<D>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
+    RI_CUDA(cudaFuncSetAttribute(resattn_prefix_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+    RI_CUDA(cudaFuncSetAttribute(resattn_prefix_kernel<D, NT>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
     attr_done[dev] = true;
   }
-  const int row_tiles = (p.batch * p.group + C::kRows - 1) / C::kRows;
+  const int rows_per_cta = NT * C::kRows;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(prefix_splits, p.hkv * row_tiles);
+  cfg.gridDim = dim3(prefix_splits, p.hkv * ((p.batch * p.group + rows_per_cta - 1) / rows_per_cta));
   cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = C::kSmemBytes;
   cfg.stream = st;
@@ -493,5 +517,13 @@ int launch_prefix(const AttnParams& p, int prefix_splits, cudaStream_t st) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, resattn_prefix_kernel<D>, p), "shared-prefix attention launch");
+  return cuda_status(cudaLaunchKernelEx(&cfg, resattn_prefix_kernel<D, NT>, p), "shared-prefix attention launch");
+}
+
+template <int D>
+int launch_prefix(const AttnParams& p, int prefix_splits, cudaStream_t st) {
+  if constexpr (D == 128) {
+    if (p.batch * p.group > 128) return launch_prefix_tiles<128, 2>(p, prefix_splits, st);
+  }
+  return launch_prefix_tiles<D, 1>(p, prefix_splits, st);
 }
