@@ -51,7 +51,7 @@ struct AttnParams {
   int32_t* status;
   // shared-prefix decode only
   int prefix_len, prefix_splits;           // tokens of the prefix, pieces its launch cuts it into (0: no such launch)
-  int steps_per_split;                     // 64-token steps of a piece
+  int steps_per_split;                     // steps of a piece
   int max_tokens;                          // what a block table row can hold
   int kv_begin;                            // first token of the second launch (the prefix's length, or 0)
   const int32_t* prefix_table;             // page table row that holds the prefix
@@ -292,7 +292,7 @@ extern "C" int ri_resattn_decode_shared_prefix(
   RI_CHECK_ARG(group == 4 || group == 6 || group == 8,
                "decode residue Q8/Q16 supports logical GQA ratios (4, 6, 8), got %d", group);
   RI_CHECK_ARG(page_size >= 16 && page_size % 16 == 0, "page size must be a multiple of 16, got %d", page_size);
-  RI_CHECK_ARG(batch >= 0 && batch <= 65535 && num_pages > 0 && bt_cols >= 1 && bt_stride >= 0 && num_kv_heads <= 65535,
+  RI_CHECK_ARG(batch >= 0 && batch <= 65535 && num_pages > 0 && num_pages < (int64_t(1) << 31) && bt_cols >= 1 && bt_stride >= 0 && num_kv_heads <= 65535,
                "bad batch / page pool / block table");
   const int64_t cap = bt_cols * page_size;
   RI_CHECK_ARG(cap < (int64_t(1) << 31) - 256, "a block table of %lld tokens is too long", (long long)cap);
@@ -318,8 +318,8 @@ extern "C" int ri_resattn_decode_shared_prefix(
                  reinterpret_cast<uintptr_t>(v_sf) | reinterpret_cast<uintptr_t>(q_bf16) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
                "q, out and the KV pool must be 16-byte aligned");
   const int64_t need = ri_resattn_shared_prefix_workspace_bytes(batch, num_q_heads, head_dim, prefix_splits, splits);
-  RI_CHECK_ARG(batch == 0 || (workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
-               "%d + %d splits need a 16-byte aligned workspace of %lld bytes, got %lld", prefix_splits, splits, (long long)need,
+  RI_CHECK_ARG(batch == 0 || (workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 31) == 0),
+               "%d + %d splits need a 32-byte aligned workspace of %lld bytes, got %lld", prefix_splits, splits, (long long)need,
                (long long)workspace_bytes);
   if (batch == 0) return RI_OK;
   DeviceInfo di;
@@ -344,7 +344,8 @@ extern "C" int ri_resattn_decode_shared_prefix(
   p.kv_begin = prefix_splits > 0 ? prefix_len : 0;
   p.max_tokens = int(cap);
   {
-    const int64_t steps = (int64_t(prefix_len) + 63) / 64;
+    const int step = head_dim == 128 ? tcattn::PxCfg<128>::kStep : tcattn::PxCfg<256>::kStep;
+    const int64_t steps = (int64_t(prefix_len) + step - 1) / step;
     p.steps_per_split = prefix_splits > 0 ? int((steps + prefix_splits - 1) / prefix_splits) : 0;
     // tiles from the one that holds token kv_begin to the longest sequence's last one
     const int64_t bound = max_kv_len > 0 && max_kv_len < cap ? max_kv_len : cap;

@@ -997,16 +997,16 @@ resattn_pv_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
 }
 
 // 3-D byte tensor over a code pool: [pages, rows of a page = heads * page_size, D/2 bytes], pages `page_stride`
-// bytes apart; box = one 128-token tile; swizzle = the operand swizzle of the scores' MMA (64 bytes for head_dim
+// bytes apart; box = one 128-token tile (or `rows` tokens); swizzle = the operand swizzle of the scores' MMA (64 bytes for head_dim
 // 128, 128 bytes for 256)
 template <int D>
-int make_pool_map(CUtensorMap* map, const uint8_t* base, int64_t pages, int64_t page_rows, int64_t page_stride) {
+int make_pool_map(CUtensorMap* map, const uint8_t* base, int64_t pages, int64_t page_rows, int64_t page_stride, int rows = kTile) {
   EncodeTiledFn fn;
   int s = get_encode_fn(&fn);
   if (s) return s;
   cuuint64_t dims[3] = {cuuint64_t(D / 2), cuuint64_t(page_rows), cuuint64_t(pages)};
   cuuint64_t strides[2] = {cuuint64_t(D / 2), cuuint64_t(page_stride)};
-  cuuint32_t box[3] = {cuuint32_t(D / 2), cuuint32_t(kTile), 1};
+  cuuint32_t box[3] = {cuuint32_t(D / 2), cuuint32_t(rows), 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, D == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,

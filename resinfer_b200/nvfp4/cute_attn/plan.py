@@ -134,14 +134,11 @@ def select_shared_prefix_plan(batch, num_kv_heads, group, prefix_len, max_kv_len
     prefix (128 query rows of one KV head each; 0 = no launch of its own) and of the tokens behind it."""
     _check_output_dimension(head_dim, False)
     ctas_per_sm = 2 if head_dim == 128 else 1
-    slots = sm_count * ctas_per_sm
-    steps = -(-prefix_len // 64)
-    rows = batch * group
-    tiles = 2 if head_dim == 128 and rows > 128 else 1     # 128-row tiles of a CTA; two leave room for one CTA per SM
-    units = max(1, num_kv_heads * -(-rows // (128 * tiles)))
+    steps = -(-prefix_len // (128 if head_dim == 128 else 64))
+    units = max(1, num_kv_heads * -(-(batch * group) // 128))
     prefix_splits = 0
     if steps:
-        piece = max(2, -(-steps // max(1, slots // tiles // units)))
+        piece = max(1, -(-steps // max(1, sm_count // units)))
         prefix_splits = min(256, -(-steps // piece))
     rest = max(0, max_kv_len - (prefix_len // 128 * 128 if prefix_splits else 0))
     return prefix_splits, _select_splits(batch, num_kv_heads, rest, sm_count, ctas_per_sm=ctas_per_sm)
