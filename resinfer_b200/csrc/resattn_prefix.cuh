@@ -17,18 +17,19 @@
 // Rows shorter than the prefix are masked at their own length; rows beyond the batch have length zero.
 //
 // What bounds it: the special function unit, 16 exponentials a cycle and SM -- 1024 cycles for 128 x 128 scores, against
-// 128 + 256 for the two products.  So the two softmax warps of a scheduler, one of each group, take turns at it: one
-// computes its 128 exponentials per thread while the other has its waits, loads, maxima and stores.  (Without turns all
-// softmax warps arrive at the exponentials together and the unit rests while all of them wait; measured with two, four
-// and eight warps a scheduler, 64-token steps: 1.0 us a step instead of the 0.6 us that the arithmetic takes.)
+// 128 + 256 for the two products -- and, close behind, issue slots and the latencies of the chain scores -> P -> product.
+// So the two softmax groups run free of each other: a group takes a step's exponentials with the maximum that it knows,
+// raised where the step itself shows a row grown beyond 2^8 times it; what the other group raised meanwhile is seen once the
+// products of the step in front are complete, and P is then scaled by the difference -- exactly, maxima being whole powers
+// of two.  (Waiting for the other group's maximum first, or taking turns at the exponentials, cost more than it hid.)
 //
-// Roles (20 warps):
+// Roles (16 warps):
 //   0-3, 4-7   softmax, thread = row (tensor-memory lane); the first group takes the even steps, the second the odd ones
-//   8-15       V conversion: codes x scales -> FP16 in the 128-byte-swizzled N-major operand layout
-//   16, 17     one thread each issues the scores' and the P.V products
-//   18         copies: tiled TMA for the codes (in the operand swizzle), bulk copies for the scales, one lane per run of
+//   8-11       V conversion: codes x scales -> FP16 in the 128-byte-swizzled N-major operand layout
+//   12, 13     one thread each issues the scores' and the P.V products
+//   14         copies: tiled TMA for the codes (in the operand swizzle), bulk copies for the scales, one lane per run of
 //              tokens that lie together in a page (pages of 16 tokens and up)
-//   19         K scales into the layout of the copies to tensor memory (by itself: behind the V conversion, which waits for
+//   15         K scales into the layout of the copies to tensor memory (by itself: behind the V conversion, which waits for
 //              products three steps back, it held the scores up)
 // Every wait is bounded.  A role whose wait expires sets the abort flag, which ends all other waits at once, and runs on
 // through its loop (every address is in bounds whatever the data), so all roles meet at the end and the status word is set.
@@ -36,8 +37,8 @@ template <int D>
 struct PxCfg {
   static constexpr int kStep = D == 128 ? 128 : 64;            // tokens per step
   static constexpr int kRows = 128;
-  static constexpr int kFirstConv = 8, kQkWarp = 16, kPvWarp = 17, kProdWarp = 18, kScaleWarp = 19;
-  static constexpr int kThreads = 640;
+  static constexpr int kFirstConv = 8, kConv = 4, kQkWarp = 12, kPvWarp = 13, kProdWarp = 14, kScaleWarp = 15;
+  static constexpr int kThreads = 512;
   static constexpr int kStages = 4;
   static constexpr int kMma = D / 64;
   static constexpr int kRowBytes = D / 2;
@@ -106,18 +107,12 @@ __device__ __forceinline__ void unpair64(uint64_t v, float& lo, float& hi) {
 }
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t d;
-  asm volatile("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t d;
-  asm volatile("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ void ex2_inplace(float& v) { asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(v)); }
-__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
-  uint32_t d;
-  asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -134,10 +129,10 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
   constexpr int S = C::kStages, kStep = C::kStep;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[S], bar_empty[S], bar_kready[S];
-  __shared__ __align__(8) uint64_t bar_sfull[2], bar_sfree[2], bar_pready[2], bar_pvdone[2], bar_vready[2], bar_vfree[2], bar_max[2][4];
+  __shared__ __align__(8) uint64_t bar_sfull[2], bar_sfree[2], bar_pready[2], bar_pvdone[2], bar_vready[2], bar_vfree[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
-  __shared__ float row_m[C::kRows], row_l[C::kRows];           // running maximum; row sums of the second group
+  __shared__ float row_m[C::kRows], row_l[C::kRows];           // running maxima; row sums of the second group
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.x, hkv = blockIdx.y % p.hkv, row0 = (blockIdx.y / p.hkv) * C::kRows;
@@ -159,16 +154,15 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
     for (int s = 0; s < S; ++s) {
       mbar_init(smem_u32(&bar_full[s]), 1);
       mbar_init(smem_u32(&bar_kready[s]), 1);
-      mbar_init(smem_u32(&bar_empty[s]), 8 + 1);               // conversion warps + the commit of the scores' MMAs
+      mbar_init(smem_u32(&bar_empty[s]), C::kConv + 1);               // conversion warps + the commit of the scores' MMAs
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(smem_u32(&bar_sfull[s]), 1);
       mbar_init(smem_u32(&bar_sfree[s]), 4);
       mbar_init(smem_u32(&bar_pready[s]), 4);
       mbar_init(smem_u32(&bar_pvdone[s]), 1);
-      mbar_init(smem_u32(&bar_vready[s]), 8);
+      mbar_init(smem_u32(&bar_vready[s]), C::kConv);
       mbar_init(smem_u32(&bar_vfree[s]), 1);
-      for (int q = 0; q < 4; ++q) mbar_init(smem_u32(&bar_max[s][q]), 1);
     }
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -208,19 +202,18 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
 
   if (warp < C::kFirstConv) {
     // ============================================================ softmax warps
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     const int grp = warp >> 2, quarter = warp & 3;
     const uint32_t lane_base = tmem_base + (uint32_t(quarter * 32) << 16);
     const uint32_t s_col = lane_base + C::kColS + grp * kStep;
     const uint32_t b_sfull = smem_u32(&bar_sfull[grp]), b_sfree = smem_u32(&bar_sfree[grp]), b_pready = smem_u32(&bar_pready[grp]);
     const uint32_t b_pvdone = smem_u32(&bar_pvdone[grp ^ 1]);  // of the steps of the other group, in front of this group's
-    const uint32_t b_max_mine = smem_u32(&bar_max[grp][quarter]), b_max_other = smem_u32(&bar_max[grp ^ 1][quarter]);
     const int r = quarter * 32 + lane, row = row0 + r;
     int lim = 0;
     if (row < rows) lim = min(max(__ldg(p.seq_lens + row / G), 0), p.prefix_len);
-    const int lim_min = __reduce_min_sync(0xffffffffu, lim), lim_max = __reduce_max_sync(0xffffffffu, lim);
+    const int lim_max = __reduce_max_sync(0xffffffffu, lim);
     const float scale = p.score_scale_log2;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f;                              // this group's: the row's maximum as it last knew it, its row sum
     if (lim_max <= s_begin * kStep) {
       // none of these rows reaches the split's tokens: their P is zero throughout
       if (grp == 0) {
@@ -243,9 +236,21 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
       }
     } else {
       for (int j = grp, k = 0; j < steps; j += 2, ++k) {
+        const int left = lim - (s_begin + j) * kStep;          // of this row's tokens, from this step on
         px_wait(b_sfull, k & 1, &abort_flag, 5);
         __syncwarp();
         tc_fence_after();
+        if (__any_sync(0xffffffffu, left < kStep)) {           // a row ends here: its scores beyond are -inf
+#pragma unroll 1
+          for (int c = 0; c < kStep; c += 16) {
+            float t[16];
+            tmem_ld16(s_col + c, t);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) t[i] = c + i < left ? t[i] : -INFINITY;
+            tmem_st16f(s_col + c, t);
+          }
+          tmem_wait_st();
+        }
         uint32_t s[kStep / 32][32];
 #pragma unroll
         for (int c = 0; c < kStep / 32; ++c) tmem_ld32_async(s_col + 32 * c, s[c]);
@@ -254,79 +259,62 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(b_sfree);                   // step j+2's scores may overwrite S
-        const int tok0 = (s_begin + j) * kStep;
-        if (tok0 + kStep > lim_min) {
-#pragma unroll
-          for (int i = 0; i < kStep; ++i)
-            if (tok0 + i >= lim) s[i >> 5][i & 31] = 0xff800000u;   // -inf
-        }
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < kStep; i += 2)
           m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(s[i >> 5][i & 31]), __uint_as_float(s[i >> 5][(i & 31) + 1]));
         const float mx = max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]) * scale;   // scale > 0
-        // the running maximum goes from group to group, step by step
-        float before = -INFINITY;
-        if (j > 0) {
-          px_wait(b_max_other, ((j - 1) >> 1) & 1, &abort_flag, 10);
-          before = row_m[r];
-        }
-        const float now = mx > before + kLazyThreshold ? mx : before;
-        row_m[r] = now;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(b_max_mine);
-        if (now != m) {                                        // this group's row sums follow
-          l *= m == -INFINITY ? 0.f : fast_exp2(m - now);
-          m = now;
-        }
-        const float f = before == -INFINITY ? 0.f : fast_exp2(before - now);
-        const bool grown = __any_sync(0xffffffffu, now != before) && j > 0;
-        const float mu = m == -INFINITY ? 0.f : m;             // a row with nothing to attend to yet
+        const float m_try = mx > m + kLazyThreshold ? ceilf(mx) : m;
+        const float mu = m_try == -INFINITY ? 0.f : m_try;     // a row with nothing to attend to yet
         const uint64_t scale2 = pair64(__float_as_uint(scale), __float_as_uint(scale));
         const uint64_t mu2 = pair64(__float_as_uint(-mu), __float_as_uint(-mu));
         uint64_t sum[2] = {0, 0};
         uint32_t pk[kStep / 2];
-        if (j > 0) asm volatile("bar.sync %0, 64;" ::"r"(1 + warp) : "memory");     // this warp's turn
-        // Pair i's exponentials are issued, pair i-kLag's are summed and packed (their results are there by then) and pair
-        // i+2's arguments are formed: one warp keeps the unit busy.  The order is this one: everything is volatile.
-        constexpr int kPairs = kStep / 2, kLag = 4;
-        uint64_t x[kPairs];
-        float e[kPairs][2];
 #pragma unroll
-        for (int i = -2; i < kPairs + kLag; ++i) {
-          if (i + 2 < kPairs) x[i + 2] = fma2(pair64(s[(i + 2) >> 4][(2 * i + 4) & 31], s[(i + 2) >> 4][(2 * i + 5) & 31]), scale2, mu2);
-          if (i >= 0 && i < kPairs) {
-            unpair64(x[i], e[i][0], e[i][1]);
-            ex2_inplace(e[i][0]);
-            ex2_inplace(e[i][1]);
-          }
-          if (i >= kLag) {
-            const int o = i - kLag;
-            sum[o & 1] = add2(sum[o & 1], pair64(__float_as_uint(e[o][0]), __float_as_uint(e[o][1])));
-            pk[o] = pack_h2(e[o][0], e[o][1]);
-          }
+        for (int i = 0; i < kStep / 2; ++i) {
+          float a, b;
+          unpair64(fma2(pair64(s[i >> 4][(2 * i) & 31], s[i >> 4][(2 * i + 1) & 31]), scale2, mu2), a, b);
+          a = fast_exp2(a);
+          b = fast_exp2(b);
+          sum[i & 1] = add2(sum[i & 1], pair64(__float_as_uint(a), __float_as_uint(b)));
+          pk[i] = h2_bits(__floats2half2_rn(a, b));
         }
-        if (j + 1 < steps) asm volatile("bar.arrive %0, 64;" ::"r"(1 + (warp ^ 4)) : "memory");   // the other group's turn
+        float l_step;
         {
           float a, b;
           unpair64(add2(sum[0], sum[1]), a, b);
-          l += a + b;
+          l_step = a + b;
         }
-        if (j > 0) {                                           // P is free, and the accumulator complete up to step j-1
+        float before = -INFINITY;
+        if (j > 0) {                                           // P is free, the accumulator and row_m those of step j-1
           px_wait(b_pvdone, ((j - 1) >> 1) & 1, &abort_flag, 7);
           __syncwarp();
           tc_fence_after();
+          before = row_m[r];
         }
-        if (grown) {                                           // rescale this row's accumulator in place
-#pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
-            float o[16];
-            tmem_ld16(lane_base + C::kColO + c, o);
+        if (__any_sync(0xffffffffu, m_try != before || m != before)) {   // a maximum has moved, here or in the other group
+          const float now = mx > before + kLazyThreshold ? ceilf(mx) : before;
+          const float f_o = before == -INFINITY ? 0.f : fast_exp2(before - now);
+          const float f_p = m_try == -INFINITY ? 0.f : fast_exp2(m_try - now);   // powers of two, 1 at most 2^8
+          l *= m == -INFINITY ? 0.f : fast_exp2(m - now);
+          l_step *= f_p;
+          const __half2 f2 = __float2half2_rn(f_p);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] *= f;
-            tmem_st16f(lane_base + C::kColO + c, o);
+          for (int i = 0; i < kStep / 2; ++i) pk[i] = h2_bits(__hmul2(bits_h2(pk[i]), f2));
+          if (j > 0) {
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              float o[16];
+              tmem_ld16(lane_base + C::kColO + c, o);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] *= f_o;
+              tmem_st16f(lane_base + C::kColO + c, o);
+            }
           }
+          m = now;
+          row_m[r] = now;
         }
+        l += l_step;
 #pragma unroll
         for (int c = 0; c < kStep / 2; c += 32) tmem_st32(lane_base + C::kColP + c, pk + c);
         tmem_wait_st();
@@ -338,13 +326,14 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
     // ---------------------------------------------------------------- the rows' partials: half of the columns per group
     if (steps > 0) px_wait(smem_u32(&bar_pvdone[(steps - 1) & 1]), ((steps - 1) >> 1) & 1, &abort_flag, 12);
     const float m_end = steps > 0 && lim_max > s_begin * kStep ? row_m[r] : -INFINITY;   // ordered by the products in between
-    if (grp == 1) row_l[r] = m == -INFINITY ? 0.f : l * fast_exp2(m - m_end);
+    l = m == -INFINITY ? 0.f : l * fast_exp2(m - m_end);
+    if (grp == 1) row_l[r] = l;
     asm volatile("bar.sync %0, 64;" ::"r"(9 + quarter) : "memory");
     if (__any_sync(0xffffffffu, row < rows)) {                 // whole warps: the loads from tensor memory are collective
       const int b = row / G, g = row - b * G;
       const int64_t slot = (int64_t(p.splits + split) * p.batch + b) * p.hq + hkv * G + g;
       if (grp == 0 && row < rows) {
-        p.l_part[slot] = m_end == -INFINITY ? 0.f : (m == -INFINITY ? 0.f : l * fast_exp2(m - m_end)) + row_l[r];
+        p.l_part[slot] = m_end == -INFINITY ? 0.f : l + row_l[r];
         p.m_part[slot] = m_end;
       }
       if (__any_sync(0xffffffffu, row < rows && m_end != -INFINITY)) {
@@ -367,50 +356,60 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
     }
   } else if (warp < C::kQkWarp) {
     // ============================================================ V conversion warps: 32 tokens x 64 head-dim values each
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     const int cw = warp - C::kFirstConv;
-    const int tok = 32 * (cw / C::kDBlocks) + lane, dblk = cw % C::kDBlocks;
+    constexpr int kUnits = kStep / 32 * C::kDBlocks / C::kConv;   // 32 tokens x 64 values each
     for (int j = 0, stg = 0, ph = 0; j < steps; ++j, stg = (stg + 1 == S ? 0 : stg + 1), ph ^= (stg == 0)) {
       const int vb = j & 1;
       px_wait(smem_u32(&bar_full[stg]), ph, &abort_flag, 6);
       const uint8_t* st = stage0 + stg * C::kStageBytes;
-      uint4 c0 = make_uint4(0, 0, 0, 0), c1 = c0;
-      uint32_t sfw = 0;
-      if ((s_begin + j) * kStep + tok < p.prefix_len) {
-        const uint8_t* src = st + C::kStgV;
-        c0 = *reinterpret_cast<const uint4*>(src + swz_off<D>(tok, 32 * dblk));
-        c1 = *reinterpret_cast<const uint4*>(src + swz_off<D>(tok, 32 * dblk + 16));
-        sfw = *reinterpret_cast<const uint32_t*>(st + C::kStgVsf + tok * C::kSfPerRow + dblk * 4);
+      uint4 c0[kUnits], c1[kUnits];
+      uint32_t sfw[kUnits];
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const int unit = cw * kUnits + u, tok = 32 * (unit / C::kDBlocks) + lane, dblk = unit % C::kDBlocks;
+        c0[u] = c1[u] = make_uint4(0, 0, 0, 0);
+        sfw[u] = 0;
+        if ((s_begin + j) * kStep + tok < p.prefix_len) {
+          const uint8_t* src = st + C::kStgV;
+          c0[u] = *reinterpret_cast<const uint4*>(src + swz_off<D>(tok, 32 * dblk));
+          c1[u] = *reinterpret_cast<const uint4*>(src + swz_off<D>(tok, 32 * dblk + 16));
+          sfw[u] = *reinterpret_cast<const uint32_t*>(st + C::kStgVsf + tok * C::kSfPerRow + dblk * 4);
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bar_empty[stg]));   // the codes are in registers: the stage may be refilled
       if (j >= 2) px_wait(smem_u32(&bar_vfree[vb]), ((j >> 1) - 1) & 1, &abort_flag, 11);
-      const uint32_t words[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-      uint32_t lo, hi, sc2[4];                                 // the four block scales as FP16 pairs (s, s)
-      asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-          : "=r"(lo), "=r"(hi) : "r"(sfw));
-      sc2[0] = __byte_perm(lo, 0, 0x1010); sc2[1] = __byte_perm(lo, 0, 0x3232);
-      sc2[2] = __byte_perm(hi, 0, 0x1010); sc2[3] = __byte_perm(hi, 0, 0x3232);
-      const uint32_t dst0 = smem_u32(smem + C::kOffV + vb * C::kVBytes + dblk * (kStep * 128) + (tok >> 3) * 1024 + (tok & 7) * 128) |
-                            ((tok & 7) << 4);
 #pragma unroll
-      for (int w8 = 0; w8 < 8; ++w8) {                         // one 16-byte chunk = 8 FP16 per code word
-        uint32_t h0, h1, h2, h3;
-        asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
-            : "=r"(h0), "=r"(h1), "=r"(h2), "=r"(h3) : "r"(words[w8]));
-        const __half2 s2 = bits_h2(sc2[w8 >> 1]);
-        const uint32_t o0 = h2_bits(__hmul2(bits_h2(h0), s2)), o1 = h2_bits(__hmul2(bits_h2(h1), s2));
-        const uint32_t o2 = h2_bits(__hmul2(bits_h2(h2), s2)), o3 = h2_bits(__hmul2(bits_h2(h3), s2));
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst0 ^ (w8 << 4)), "r"(o0), "r"(o1), "r"(o2), "r"(o3) : "memory");
+      for (int u = 0; u < kUnits; ++u) {
+        const int unit = cw * kUnits + u, tok = 32 * (unit / C::kDBlocks) + lane, dblk = unit % C::kDBlocks;
+        const uint32_t words[8] = {c0[u].x, c0[u].y, c0[u].z, c0[u].w, c1[u].x, c1[u].y, c1[u].z, c1[u].w};
+        uint32_t lo, hi, sc2[4];                               // the four block scales as FP16 pairs (s, s)
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+            : "=r"(lo), "=r"(hi) : "r"(sfw[u]));
+        sc2[0] = __byte_perm(lo, 0, 0x1010); sc2[1] = __byte_perm(lo, 0, 0x3232);
+        sc2[2] = __byte_perm(hi, 0, 0x1010); sc2[3] = __byte_perm(hi, 0, 0x3232);
+        const uint32_t dst0 = smem_u32(smem + C::kOffV + vb * C::kVBytes + dblk * (kStep * 128) + (tok >> 3) * 1024 + (tok & 7) * 128) |
+                              ((tok & 7) << 4);
+#pragma unroll
+        for (int w8 = 0; w8 < 8; ++w8) {                       // one 16-byte chunk = 8 FP16 per code word
+          uint32_t h0, h1, h2, h3;
+          asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+              "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+              "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+              : "=r"(h0), "=r"(h1), "=r"(h2), "=r"(h3) : "r"(words[w8]));
+          const __half2 s2 = bits_h2(sc2[w8 >> 1]);
+          const uint32_t o0 = h2_bits(__hmul2(bits_h2(h0), s2)), o1 = h2_bits(__hmul2(bits_h2(h1), s2));
+          const uint32_t o2 = h2_bits(__hmul2(bits_h2(h2), s2)), o3 = h2_bits(__hmul2(bits_h2(h3), s2));
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst0 ^ (w8 << 4)), "r"(o0), "r"(o1), "r"(o2), "r"(o3) : "memory");
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bar_vready[vb]));
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == C::kQkWarp) {
       // ============================================================ scores
       const uint32_t idesc_qk = (1u << 7) | (1u << 10) | (uint32_t(kStep >> 3) << 17) | (uint32_t(C::kRows >> 4) << 24);
