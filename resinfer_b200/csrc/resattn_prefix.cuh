@@ -26,18 +26,17 @@
 // Roles (16 warps):
 //   0-3, 4-7   softmax, thread = row (tensor-memory lane); the first group takes the even steps, the second the odd ones
 //   8-11       V conversion: codes x scales -> FP16 in the 128-byte-swizzled N-major operand layout
-//   12, 13     one thread each issues the scores' and the P.V products
-//   14         copies: tiled TMA for the codes (in the operand swizzle), bulk copies for the scales, one lane per run of
-//              tokens that lie together in a page (pages of 16 tokens and up)
-//   15         K scales into the layout of the copies to tensor memory (by itself: behind the V conversion, which waits for
-//              products three steps back, it held the scores up)
+//   12, 13     one thread each issues the scores' and the P.V products; warp 12 lays K's scales out for them
+//   14, 15     copies of codes (tiled TMA in the operand swizzle) and of scales (bulk), one lane per run of tokens that lie
+//              together in a page.  A small copy costs its issuer about 50 cycles: with pages of 16 tokens one warp for all
+//              32 copies of a step took 1.8 us a step.
 // Every wait is bounded.  A role whose wait expires sets the abort flag, which ends all other waits at once, and runs on
 // through its loop (every address is in bounds whatever the data), so all roles meet at the end and the status word is set.
 template <int D>
 struct PxCfg {
   static constexpr int kStep = D == 128 ? 128 : 64;            // tokens per step
   static constexpr int kRows = 128;
-  static constexpr int kFirstConv = 8, kConv = 4, kQkWarp = 12, kPvWarp = 13, kProdWarp = 14, kScaleWarp = 15;
+  static constexpr int kFirstConv = 8, kConv = 4, kQkWarp = 12, kPvWarp = 13, kProdWarp = 14;
   static constexpr int kThreads = 512;
   static constexpr int kStages = 4;
   static constexpr int kMma = D / 64;
@@ -128,7 +127,7 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
   using C = PxCfg<D>;
   constexpr int S = C::kStages, kStep = C::kStep;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bar_full[S], bar_empty[S], bar_kready[S];
+  __shared__ __align__(8) uint64_t bar_full[S], bar_empty[S];
   __shared__ __align__(8) uint64_t bar_sfull[2], bar_sfree[2], bar_pready[2], bar_pvdone[2], bar_vready[2], bar_vfree[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
@@ -152,8 +151,7 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(smem_u32(&bar_full[s]), 1);
-      mbar_init(smem_u32(&bar_kready[s]), 1);
+      mbar_init(smem_u32(&bar_full[s]), 2);                    // codes, scales
       mbar_init(smem_u32(&bar_empty[s]), C::kConv + 1);               // conversion warps + the commit of the scores' MMAs
     }
     for (int s = 0; s < 2; ++s) {
@@ -414,19 +412,32 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
       // ============================================================ scores
       const uint32_t idesc_qk = (1u << 7) | (1u << 10) | (uint32_t(kStep >> 3) << 17) | (uint32_t(C::kRows >> 4) << 24);
       constexpr uint32_t kSbo = 8 * C::kRowBytes, kLayout = D == 128 ? 4u : 2u;
+      const uint64_t q_desc = desc_kmajor(smem_u32(smem), kSbo, kLayout);
+      const uint64_t k_desc0 = desc_kmajor(smem_u32(stage0), kSbo, kLayout), ksf_desc0 = desc_sf(smem_u32(stage0) + C::kStgKsf);
+      const uint32_t sfq = tmem_base + C::kColSfq;
       if (elect_one()) {
-        const uint64_t q_desc = desc_kmajor(smem_u32(smem), kSbo, kLayout);
-        const uint64_t k_desc0 = desc_kmajor(smem_u32(stage0), kSbo, kLayout), ksf_desc0 = desc_sf(smem_u32(stage0) + C::kStgKsf);
-        const uint32_t sfq = tmem_base + C::kColSfq;
 #pragma unroll
         for (int i = 0; i < 2 * C::kMma; ++i)                  // the query scales, once
           tmem_cp_sf(sfq + 4 * i, desc_sf(smem_u32(smem) + C::kOffQsf + i * 512));
-        for (int j = 0, stg = 0, ph = 0; j < steps; ++j, stg = (stg + 1 == S ? 0 : stg + 1), ph ^= (stg == 0)) {
-          const int sb = j & 1;
-          px_wait(smem_u32(&bar_full[stg]), ph, &abort_flag, 3);
-          px_wait(smem_u32(&bar_kready[stg]), ph, &abort_flag, 14);
-          if (j >= 2) px_wait(smem_u32(&bar_sfree[sb]), ((j >> 1) - 1) & 1, &abort_flag, 4);
-          tc_fence_after();
+      }
+      __syncwarp();
+      for (int j = 0, stg = 0, ph = 0; j < steps; ++j, stg = (stg + 1 == S ? 0 : stg + 1), ph ^= (stg == 0)) {
+        const int sb = j & 1;
+        px_wait(smem_u32(&bar_full[stg]), ph, &abort_flag, 3);
+        {                                                      // [token][group] -> [group of 64 values][32 rows][4 quarters] words
+          uint8_t* st = stage0 + stg * C::kStageBytes;
+#pragma unroll
+          for (int q = 0; q < kStep / 32; ++q) {
+            const uint32_t* raw = reinterpret_cast<const uint32_t*>(st + C::kStgKraw + (32 * q + lane) * C::kSfPerRow);
+#pragma unroll
+            for (int i = 0; i < C::kMma; ++i) *reinterpret_cast<uint32_t*>(st + C::kStgKsf + 512 * i + lane * 16 + q * 4) = raw[i];
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        if (j >= 2) px_wait(smem_u32(&bar_sfree[sb]), ((j >> 1) - 1) & 1, &abort_flag, 4);
+        tc_fence_after();
+        __syncwarp();
+        if (elect_one()) {
           const uint64_t k_desc = k_desc0 + uint64_t((stg * C::kStageBytes) >> 4), ksf_desc = ksf_desc0 + uint64_t((stg * C::kStageBytes) >> 4);
           const uint32_t sfk = tmem_base + C::kColSfk + sb * 4 * C::kMma;
 #pragma unroll
@@ -436,10 +447,10 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
             mma_fp4<false>(tmem_base + C::kColS + sb * kStep, q_desc + uint64_t(((i / C::kMma) * C::kQBytes >> 4) + 2 * (i % C::kMma)),
                            k_desc + uint64_t(2 * (i % C::kMma)), idesc_qk, sfq + 4 * i, sfk + 4 * (i % C::kMma), i > 0 ? 1u : 0u);
           mma_commit(smem_u32(&bar_sfull[sb]));
-          mma_commit(smem_u32(&bar_empty[stg]));               // the K codes of the stage have been read
+          mma_commit(smem_u32(&bar_empty[stg]));               // the K codes and scales of the stage have been read
         }
+        __syncwarp();
       }
-      __syncwarp();
     } else if (warp == C::kPvWarp) {
       // ============================================================ P.V: a thread of another warp, so that the next scores do not
       // stand in line behind the exponentials
@@ -464,7 +475,8 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
         if (steps > 0) px_wait(smem_u32(&bar_pvdone[(steps - 1) & 1]), ((steps - 1) >> 1) & 1, &abort_flag, 13);   // nothing is in flight any more
       }
       __syncwarp();
-    } else if (warp == C::kProdWarp) {
+    } else {
+      const bool codes = warp == C::kProdWarp;
       // ============================================================ copies: lane i fetches the i-th run of a step.  `run` tokens
       // (a power of two up to the step, dividing the page size) lie together in a page.
       const int runs = kStep / run;
@@ -484,35 +496,23 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
         const uint32_t st = smem_u32(stage0 + stg * C::kStageBytes), full = smem_u32(&bar_full[stg]);
         if (lane == 0) {                                       // whole runs, also the one in which the prefix ends
           const int live = min(runs, (p.prefix_len - (s_begin + j) * kStep + run - 1) / run);
-          mbar_expect_tx(full, live * run * 2 * (C::kRowBytes + C::kSfPerRow));
+          mbar_expect_tx(full, live * run * 2 * (codes ? C::kRowBytes : C::kSfPerRow));
         }
         __syncwarp();
         if (lane < runs && t0 < p.prefix_len) {
           const int row = lane * run;
-          tma_load_3d(st + row * C::kRowBytes, &k_map, 0, in_row, int(page), full);
-          tma_load_3d(st + C::kStgV + row * C::kRowBytes, &v_map, 0, in_row, int(page), full);
-          const int64_t sf = page * p.sf_page_stride + int64_t(in_row) * C::kSfPerRow;
-          bulk_load_1d(st + C::kStgKraw + row * C::kSfPerRow, p.k_sf + sf, run * C::kSfPerRow, full);
-          bulk_load_1d(st + C::kStgVsf + row * C::kSfPerRow, p.v_sf + sf, run * C::kSfPerRow, full);
+          if (codes) {
+            tma_load_3d(st + row * C::kRowBytes, &k_map, 0, in_row, int(page), full);
+            tma_load_3d(st + C::kStgV + row * C::kRowBytes, &v_map, 0, in_row, int(page), full);
+          } else {
+            const int64_t sf = page * p.sf_page_stride + int64_t(in_row) * C::kSfPerRow;
+            bulk_load_1d(st + C::kStgKraw + row * C::kSfPerRow, p.k_sf + sf, run * C::kSfPerRow, full);
+            bulk_load_1d(st + C::kStgVsf + row * C::kSfPerRow, p.v_sf + sf, run * C::kSfPerRow, full);
+          }
         }
       }
       // nothing may be in flight when the CTA ends: the last stages' data have arrived
       for (int j = max(steps - S, 0); j < steps; ++j) px_wait(smem_u32(&bar_full[j % S]), (j / S) & 1, &abort_flag, 15);
-    } else {
-      // ============================================================ K scales: [token][group] -> [group][32 rows][4 quarters] words
-      for (int j = 0, stg = 0, ph = 0; j < steps; ++j, stg = (stg + 1 == S ? 0 : stg + 1), ph ^= (stg == 0)) {
-        px_wait(smem_u32(&bar_full[stg]), ph, &abort_flag, 6);
-        uint8_t* st = stage0 + stg * C::kStageBytes;
-#pragma unroll
-        for (int q = 0; q < kStep / 32; ++q) {
-          const uint32_t* raw = reinterpret_cast<const uint32_t*>(st + C::kStgKraw + (32 * q + lane) * C::kSfPerRow);
-#pragma unroll
-          for (int i = 0; i < C::kMma; ++i) *reinterpret_cast<uint32_t*>(st + C::kStgKsf + 512 * i + lane * 16 + q * 4) = raw[i];
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bar_kready[stg]));
-      }
     }
   }
   tc_fence_before();
