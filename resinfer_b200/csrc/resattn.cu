@@ -52,6 +52,7 @@ struct AttnParams {
   // shared-prefix decode only
   int prefix_len, prefix_splits;           // tokens of the prefix, pieces its launch cuts it into (0: no such launch)
   int steps_per_split;                     // steps of a piece
+  int groups_per_split;                    // groups of 16 tokens that a piece of the second launch covers
   int max_tokens;                          // what a block table row can hold
   int kv_begin;                            // first token of the second launch (the prefix's length, or 0)
   const int32_t* prefix_table;             // page table row that holds the prefix
@@ -99,6 +100,7 @@ __device__ __forceinline__ uint32_t swz_off(int row, int byte) {
 
 #include "resattn_pv.cuh"
 #include "resattn_prefix.cuh"
+#include "resattn_tail.cuh"
 }  // namespace tcattn
 
 
@@ -334,7 +336,6 @@ extern "C" int ri_resattn_decode_shared_prefix(
   p.page_shift = -1;
   for (int sft = 4; sft < 31; ++sft)
     if ((1 << sft) == page_size) p.page_shift = sft;
-  p.tma_pages = (page_size % 128 == 0 && num_pages < (int64_t(1) << 31)) ? 1 : 0;
   p.score_scale_log2 = score_scale * kLog2e;
   p.out_scale = out_scale;
   p.out = out;
@@ -347,11 +348,11 @@ extern "C" int ri_resattn_decode_shared_prefix(
     const int step = head_dim == 128 ? tcattn::PxCfg<128>::kStep : tcattn::PxCfg<256>::kStep;
     const int64_t steps = (int64_t(prefix_len) + step - 1) / step;
     p.steps_per_split = prefix_splits > 0 ? int((steps + prefix_splits - 1) / prefix_splits) : 0;
-    // tiles from the one that holds token kv_begin to the longest sequence's last one
+    // groups from the one that holds token kv_begin to the longest sequence's last one
     const int64_t bound = max_kv_len > 0 && max_kv_len < cap ? max_kv_len : cap;
-    const int64_t tiles = (bound + 127) / 128 - p.kv_begin / 128;
-    p.tiles_per_split = int((tiles + splits - 1) / splits);
-    if (p.tiles_per_split < 1) p.tiles_per_split = 1;
+    const int64_t groups = (bound + 15) / 16 - p.kv_begin / 16;
+    p.groups_per_split = int((groups + splits - 1) / splits);
+    if (p.groups_per_split < 1) p.groups_per_split = 1;
   }
   const int64_t rows = int64_t(prefix_splits + splits) * batch * num_q_heads;
   p.split_counter = static_cast<int*>(workspace);

@@ -276,97 +276,8 @@ __device__ __forceinline__ void pack_nvfp4_output(const AttnParams& p, int b, in
   }
 }
 
-// The merge of the TAIL form: this sequence's splits (ticket as above) and the partials that the prefix launch left
-// behind them, p.splits + p.prefix_splits in all, added in that order.  Every thread sums four columns over every
-// kGroups-th partial with eight 16-byte loads in flight, the groups are then added in order.
-template <int D>
-__device__ __forceinline__ void merge_tail_last_cta(const AttnParams& p, int b, int hkv, float* scratch, int* flag_sh) {
-  const int G = p.group, total = p.splits + p.prefix_splits;
-  __threadfence();
-  __syncthreads();
-  // the partials of the prefix (and the cleared tickets) are those of the launch in front of this one
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (p.splits > 1) {
-    if (threadIdx.x == 0) {
-      int* counter = p.split_counter + b * p.hkv + hkv;
-      const int last = atomicAdd(counter, 1) == p.splits - 1;
-      __threadfence();
-      *flag_sh = last;
-    }
-    __syncthreads();
-    if (!*flag_sh) return;
-  }
-  float* w_sh = scratch;                                     // [total][8] weights 2^(m_s - m), then [8] 1 / l
-  float* r_sh = w_sh + total * 8;
-  float4* red = reinterpret_cast<float4*>(r_sh + 8);         // [groups][G * D / 4]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp < G) {
-    const int head = hkv * G + warp;
-    float mm = -INFINITY;
-    for (int s = lane; s < total; s += 32) mm = fmaxf(mm, __ldcg(p.m_part + (int64_t(s) * p.batch + b) * p.hq + head));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-    float l = 0.f;
-    for (int s = lane; s < total; s += 32) {
-      const int64_t slot = (int64_t(s) * p.batch + b) * p.hq + head;
-      const float ms = __ldcg(p.m_part + slot), ls = __ldcg(p.l_part + slot);
-      const float w = ms == -INFINITY ? 0.f : fast_exp2(ms - mm);
-      w_sh[s * 8 + warp] = w;
-      l += w == 0.f ? 0.f : w * ls;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (lane == 0) r_sh[warp] = l > 0.f ? p.out_scale / l : 0.f;
-  }
-  __syncthreads();
-  const int nv = G * (D / 4), groups = min(int(blockDim.x) / nv, total);
-  const int grp = threadIdx.x / nv, c4 = threadIdx.x - grp * nv;
-  const int g = c4 / (D / 4);
-  if (grp < groups) {
-    const float4* src = reinterpret_cast<const float4*>(p.o_part + (int64_t(b) * p.hq + hkv * G) * D) + c4;
-    const int64_t stride = int64_t(p.batch) * p.hq * (D / 4);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s0 = grp; s0 < total; s0 += 8 * groups) {
-      float4 v[8];
-      float w[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int s = s0 + j * groups;
-        w[j] = s < total ? w_sh[s * 8 + g] : 0.f;
-        v[j] = w[j] != 0.f ? __ldcg(src + s * stride) : make_float4(0.f, 0.f, 0.f, 0.f);   // empty partials hold no data
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        acc.x += w[j] * v[j].x; acc.y += w[j] * v[j].y; acc.z += w[j] * v[j].z; acc.w += w[j] * v[j].w;
-      }
-    }
-    red[grp * nv + c4] = acc;
-  }
-  __syncthreads();
-  if (threadIdx.x < nv) {
-    float4 o = red[c4];
-    for (int k = 1; k < groups; ++k) {
-      const float4 a = red[k * nv + c4];
-      o.x += a.x; o.y += a.y; o.z += a.z; o.w += a.w;
-    }
-    const float r = r_sh[g];
-    o.x *= r; o.y *= r; o.z *= r; o.w *= r;
-    const int64_t oi = (int64_t(b) * p.hq + hkv * G) * D + 4 * c4;
-    if (p.out_f32) {
-      *reinterpret_cast<float4*>(static_cast<float*>(p.out) + oi) = o;
-    } else {
-      __nv_bfloat162 lo = __floats2bfloat162_rn(o.x, o.y), hi = __floats2bfloat162_rn(o.z, o.w);
-      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + oi) =
-          make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
-    }
-  }
-}
-
 // CL: the cluster reducer.  An instantiation of its own, so that the ticket form carries none of its code.
-// TAIL: the second launch of a shared-prefix decode.  It reads the tokens from p.kv_begin (the prefix's length) on, and
-// adds to its own partials the p.prefix_splits that resattn_prefix_kernel left.  Its inputs were complete when that
-// launch released this one, so only the merge waits for it.
-template <int D, bool F8, bool CL, bool TAIL = false>
+template <int D, bool F8, bool CL>
 __global__ void __launch_bounds__(PvCfg<D, F8>::kThreads, PvCfg<D, F8>::kCtasPerSm)
 resattn_pv_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                   const __grid_constant__ AttnParams p) {
@@ -403,16 +314,13 @@ resattn_pv_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   constexpr int S = kPvStages;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if constexpr (!TAIL) asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int L = min(max(__ldg(p.seq_lens + b), 0), TAIL ? p.max_tokens : int(p.bt_stride) * p.page_size);
-  // TAIL: tiles keep their absolute places, the one that holds the prefix's last token is masked below kv_begin
-  const int kv_begin = TAIL ? p.kv_begin : 0;
-  const int t_first = kv_begin / kTile;
-  const int n_tiles = !TAIL || L > kv_begin ? (L + kTile - 1) / kTile : t_first;
-  const int t_begin = min(t_first + split * p.tiles_per_split, n_tiles);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int L = min(max(__ldg(p.seq_lens + b), 0), int(p.bt_stride) * p.page_size);
+  const int n_tiles = (L + kTile - 1) / kTile;
+  const int t_begin = min(split * p.tiles_per_split, n_tiles);
   const int t_end = min(t_begin + p.tiles_per_split, n_tiles);
   const int my_tiles = t_end - t_begin;
-  if (TAIL ? my_tiles == 0 : my_tiles == 0 && p.splits > 1 && !(p.q_pack && split == 0)) {
+  if (my_tiles == 0 && p.splits > 1 && !(p.q_pack && split == 0)) {
     // nothing to read for this split: publish an empty partial and, if this CTA happens to draw the last
     // ticket, merge the others' (the whole CTA takes this branch together)
     float* scratch = reinterpret_cast<float*>(smem + kPvOffV);
@@ -429,8 +337,7 @@ resattn_pv_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         p.l_part[slot] = 0.f;
         p.m_part[slot] = -INFINITY;
       }
-      if constexpr (TAIL) merge_tail_last_cta<D>(p, b, hkv, scratch, &merge_flag);
-      else if (merge_splits_last_cta<D>(p, b, hkv, scratch, &merge_flag) && p.out_nvfp4) pack_nvfp4_output<D>(p, b, hkv, scratch);
+      if (merge_splits_last_cta<D>(p, b, hkv, scratch, &merge_flag) && p.out_nvfp4) pack_nvfp4_output<D>(p, b, hkv, scratch);
     }
     return;
   }
@@ -523,8 +430,7 @@ resattn_pv_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       float s[kHpt];
       bool mine_grows = false;
       {
-        const int at = tile * kTile + 32 * q + lane;
-        const bool valid = at < L && (!TAIL || at >= kv_begin);
+        const bool valid = tile * kTile + 32 * q + lane < L;
         if constexpr (kHpt == 8) {
           float r[16];
           tmem_ld16(lane_base + kColS + sb * 16, r);
@@ -822,8 +728,7 @@ resattn_pv_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       asm volatile("bar.sync 3, %0;" ::"n"(kPvConv * 32) : "memory");
       if (!conv_go[vb]) break;
       const uint8_t* st = stage0 + stg * C::kStageBytes;
-      const int at = (t_begin + i) * kTile + tok;
-      const bool valid = at < L && (!TAIL || at >= kv_begin);
+      const bool valid = (t_begin + i) * kTile + tok < L;
       uint4 c0 = make_uint4(0, 0, 0, 0), c1 = c0;
       uint32_t sfw = 0;
       if (valid) {
@@ -956,7 +861,7 @@ resattn_pv_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         if (g >= G) break;
         const float l = (red_l[g] + red_l[8 + g]) + (red_l[16 + g] + red_l[24 + g]);
         const int head = hkv * G + g;
-        if (!TAIL && p.splits == 1) {
+        if (p.splits == 1) {
           const float rr = l > 0.f ? p.out_scale / l : 0.f;
           const int64_t oi = (int64_t(b) * p.hq + head) * D + d;
           if (p.out_nvfp4) stage_out[g * D + d] = o_acc[g] * rr;
@@ -984,9 +889,8 @@ resattn_pv_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   // every CTA takes its ticket, also one whose waits expired (the status word flags that call), so that
   // the counters are back at zero when the grid has finished
   bool pack = p.out_nvfp4 && p.splits == 1;
-  if (TAIL || p.splits > 1) {
-    if constexpr (TAIL) merge_tail_last_cta<D>(p, b, hkv, stage_out, &merge_flag), pack = false;
-    else if constexpr (CL) merge_splits_cluster<D>(p, b, hkv, stage_out, split);
+  if (p.splits > 1) {
+    if constexpr (CL) merge_splits_cluster<D>(p, b, hkv, stage_out, split);
     else pack = merge_splits_last_cta<D>(p, b, hkv, stage_out, &merge_flag) && p.out_nvfp4;
   }
   if (pack) pack_nvfp4_output<D>(p, b, hkv, stage_out);
@@ -1043,43 +947,6 @@ int prepare_decode_pv() {
     attr_done[dev] = true;
   }
   return RI_OK;
-}
-
-// the second launch of a shared-prefix decode (or, without a prefix launch in front, the whole decode)
-template <int D>
-int launch_tail(const AttnParams& p, cudaStream_t st) {
-  using PC = PvCfg<D, false>;
-  static bool attr_done[64] = {};
-  int dev = 0;
-  RI_CUDA(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64) dev = 0;
-  auto* kernel = resattn_pv_kernel<D, false, false, true>;
-  if (!attr_done[dev]) {
-    RI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PC::kSmemBytes));
-    RI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
-    attr_done[dev] = true;
-  }
-  CUtensorMap k_map{}, v_map{};
-  if (p.tma_pages) {
-    const int64_t page_rows = int64_t(p.hkv) * p.page_size;
-    int s = make_pool_map<D>(&k_map, p.k_data, p.num_pages, page_rows, p.code_page_stride);
-    if (s) return s;
-    s = make_pool_map<D>(&v_map, p.v_data, p.num_pages, page_rows, p.code_page_stride);
-    if (s) return s;
-  }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.splits, p.hkv, p.batch);
-  cfg.blockDim = dim3(PC::kThreads);
-  cfg.dynamicSmemBytes = PC::kSmemBytes;
-  cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  if (p.prefix_splits > 0) {      // released by the prefix launch; without one, the kernel has no wait in front of its inputs
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-  }
-  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, k_map, v_map, p), "shared-prefix decode launch");
 }
 
 template <int D, bool F8>

@@ -133,15 +133,17 @@ def select_shared_prefix_plan(batch, num_kv_heads, group, prefix_len, max_kv_len
     """(prefix_splits, splits) for a decode whose sequences share their first ``prefix_len`` tokens: the pieces of the
     prefix (128 query rows of one KV head each; 0 = no launch of its own) and of the tokens behind it."""
     _check_output_dimension(head_dim, False)
-    ctas_per_sm = 2 if head_dim == 128 else 1
     steps = -(-prefix_len // (128 if head_dim == 128 else 64))
     units = max(1, num_kv_heads * -(-(batch * group) // 128))
     prefix_splits = 0
     if steps:
         piece = max(1, -(-steps // max(1, sm_count // units)))
         prefix_splits = min(256, -(-steps // piece))
-    rest = max(0, max_kv_len - (prefix_len // 128 * 128 if prefix_splits else 0))
-    return prefix_splits, _select_splits(batch, num_kv_heads, rest, sm_count, ctas_per_sm=ctas_per_sm)
+    # the rest: four warps walk over a (sequence, KV head)'s tokens; pieces of 512 tokens or more, no more of them than run at once
+    rest = max(0, max_kv_len - (prefix_len // 16 * 16 if prefix_splits else 0))
+    slots = sm_count * (4 if head_dim == 128 else 2)
+    splits = max(1, min(-(-rest // 512), 2 * slots // max(1, batch * num_kv_heads), 64))
+    return prefix_splits, splits
 
 
 def static_compile_plans(*, output_nvfp4=False, grouped_head_tile=16, residue_fold=True, head_dim=128):
