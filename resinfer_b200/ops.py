@@ -290,44 +290,59 @@ def resattn_decode_shared_prefix(q: torch.Tensor, k_data: torch.Tensor, k_sf: to
     ``nvfp4.cute_attn.plan.select_shared_prefix_plan``.  ``workspace``: a uint8 buffer of
     ``ri_resattn_shared_prefix_workspace_bytes``; without one it comes from the caching allocator on the current stream, so
     calls on different streams, and graphs that hold them, do not share it."""
-    lib = _cabi.load()
     pages, code_stride, sf_stride, hkv, d, page = _kv_pool_args(k_data, k_sf, v_data, v_sf)
-    dev = q.device
-    b, hq, dq = q.shape
-    if (q.dtype != torch.bfloat16 or not q.is_contiguous() or dq != d or dev != k_data.device):
-        raise ValueError(f"q must be contiguous BF16 [B, H_q, {d}] on {k_data.device}")
-    if out.shape != q.shape or out.device != dev or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous {tuple(q.shape)} on {dev}")
-    if (block_tables.dtype != torch.int32 or block_tables.device != dev or block_tables.dim() != 2 or block_tables.shape[0] != b
-            or block_tables.shape[1] < 1 or block_tables.stride(1) != 1):
+    dev, shape, bt_shape = k_data.get_device(), q.shape, block_tables.shape
+    if len(shape) != 3 or shape[2] != d or q.dtype != torch.bfloat16 or not q.is_contiguous() or q.get_device() != dev:
+        raise ValueError(f"q must be contiguous BF16 [B, H_q, {d}] on cuda:{dev}")
+    b, hq, _ = shape
+    if out.shape != shape or out.get_device() != dev or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {tuple(shape)} on cuda:{dev}")
+    if (len(bt_shape) != 2 or bt_shape[0] != b or bt_shape[1] < 1 or block_tables.dtype != torch.int32 or block_tables.get_device() != dev
+            or block_tables.stride(1) != 1):
         raise ValueError("block_tables must be int32 [batch, max_pages_per_seq] on the Q device with unit column stride")
-    if seq_lens.dtype != torch.int32 or seq_lens.device != dev or tuple(seq_lens.shape) != (b,) or not seq_lens.is_contiguous():
+    if seq_lens.dtype != torch.int32 or seq_lens.get_device() != dev or seq_lens.shape != (b,) or not seq_lens.is_contiguous():
         raise ValueError("seq_lens must be contiguous int32 [batch] on the Q device")
     if b and not 0 <= prefix_row < b:
         raise ValueError(f"prefix_row {prefix_row} is not a row of the block table ({b})")
-    with _on_device(dev):
-        need = lib.ri_resattn_shared_prefix_workspace_bytes(b, hq, d, prefix_splits, splits)
+    lib, device = _cabi.load(), q.device
+    with _on_device(device):
         if workspace is None:
-            workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-        elif workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
-            raise ValueError(f"workspace must be contiguous uint8 on {dev}")
-        bt = block_tables.data_ptr()
+            need = lib.ri_resattn_shared_prefix_workspace_bytes(b, hq, d, prefix_splits, splits)
+            workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+        elif workspace.dtype != torch.uint8 or workspace.get_device() != dev or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be contiguous uint8 on cuda:{dev}")
+        bt, bt_stride = block_tables.data_ptr(), block_tables.stride(0)
         st = lib.ri_resattn_decode_shared_prefix(
             q.data_ptr(), k_data.data_ptr(), k_sf.data_ptr(), v_data.data_ptr(), v_sf.data_ptr(), pages, code_stride, sf_stride,
-            bt, block_tables.stride(0), block_tables.shape[1], bt + 4 * prefix_row * block_tables.stride(0),
-            seq_lens.data_ptr(), prefix_len, b, hq, hkv, d, page, max_kv_len, score_scale, out_scale, out.data_ptr(),
-            _cabi.torch_dtype_code(out.dtype, allow_f32=True), prefix_splits, splits, workspace.data_ptr(), workspace.numel(),
-            status_word(dev).data_ptr(), _cabi.current_stream(dev))
-    _cabi.check(st, "resattn_decode_shared_prefix")
+            bt, bt_stride, bt_shape[1], bt + 4 * prefix_row * bt_stride, seq_lens.data_ptr(), prefix_len, b, hq, hkv, d, page,
+            max_kv_len, score_scale, out_scale, out.data_ptr(),
+            _cabi.DTYPE_BF16 if out.dtype == torch.bfloat16 else _cabi.torch_dtype_code(out.dtype, allow_f32=True), prefix_splits,
+            splits, workspace.data_ptr(), workspace.numel(), status_word(device).data_ptr(), _cabi.raw_stream(dev))
+    if st:
+        _cabi.check(st, "resattn_decode_shared_prefix")
     return out
 
 
+_BYTES = (torch.uint8, torch.int8, torch.float8_e4m3fn)
+
+
 def _kv_pool_args(k_data: torch.Tensor, k_sf: torch.Tensor, v_data: torch.Tensor, v_sf: torch.Tensor):
-    """(num_pages, code stride, scale stride, Hkv, D, page_size) of a paged NVFP4 pool, shapes and devices checked."""
+    """(num_pages, code stride, scale stride, Hkv, D, page_size) of a paged NVFP4 pool, shapes and devices checked.
+    The calls that use it take a few microseconds on the device: the usual case is told by a dozen comparisons."""
+    shape, cs, ss, dev = k_data.shape, k_data.stride(), k_sf.stride(), k_data.get_device()
+    if (len(shape) == 4 and v_data.shape == shape and v_data.stride() == cs and v_sf.stride() == ss and dev >= 0
+            and dev == k_sf.get_device() == v_data.get_device() == v_sf.get_device()):
+        pages, hkv, page, half = shape
+        sf = half // 8
+        if (k_sf.shape == (pages, hkv, page, sf) and v_sf.shape == k_sf.shape and half % 8 == 0 and pages > 1
+                and cs[3] == 1 and cs[2] == half and cs[1] == page * half and cs[0] >= hkv * page * half
+                and ss[3] == 1 and ss[2] == sf and ss[1] == page * sf and ss[0] >= hkv * page * sf
+                and k_data.dtype in _BYTES and k_sf.dtype in _BYTES and v_data.dtype in _BYTES and v_sf.dtype in _BYTES):
+            return pages, cs[0], ss[0], hkv, half * 2, page
     if k_data.dim() != 4 or v_data.shape != k_data.shape or k_sf.dim() != 4 or v_sf.shape != k_sf.shape:
         raise ValueError(f"a paged NVFP4 pool is codes [pages, Hkv, page, D/2] and scales [pages, Hkv, page, D/16] for K and V, got "
                          f"{tuple(k_data.shape)} / {tuple(k_sf.shape)} and {tuple(v_data.shape)} / {tuple(v_sf.shape)}")
-    pages, hkv, page, half = k_data.shape
+    pages, hkv, page, half = shape
     if half % 8 or tuple(k_sf.shape) != (pages, hkv, page, half // 8):
         raise ValueError(f"block scales of codes {tuple(k_data.shape)} must be [pages, Hkv, page, D/16] with D a multiple of 16, got {tuple(k_sf.shape)}")
     if not k_data.is_cuda or not (k_data.device == k_sf.device == v_data.device == v_sf.device):
@@ -336,10 +351,21 @@ def _kv_pool_args(k_data: torch.Tensor, k_sf: torch.Tensor, v_data: torch.Tensor
     return pages, code_stride, sf_stride, hkv, half * 2, page
 
 
-def _check_slots(slots: torch.Tensor, device) -> int:
-    if slots.dim() != 1 or slots.dtype not in (torch.int32, torch.int64) or slots.device != device or not slots.is_contiguous():
-        raise ValueError(f"slots must be contiguous 1-D int32 or int64 on {device}, got {slots.dtype} {tuple(slots.shape)} on {slots.device}")
-    return 64 if slots.dtype == torch.int64 else 32
+def _check_slots(slots: torch.Tensor, dev: int) -> int:
+    bits = {torch.int64: 64, torch.int32: 32}.get(slots.dtype)
+    if bits is None or slots.dim() != 1 or slots.get_device() != dev or not slots.is_contiguous():
+        raise ValueError(f"slots must be contiguous 1-D int32 or int64 on cuda:{dev}, got {slots.dtype} {tuple(slots.shape)} on {slots.device}")
+    return bits
+
+
+def _check_rows(name: str, x: torch.Tensor, n: int, hkv: int, d: int, dtype: torch.dtype, dev: int):
+    """(token stride, head stride) of K or V rows."""
+    shape, st = x.shape, x.stride()
+    if (len(shape) != 3 or shape[0] < n or shape[1] != hkv or shape[2] != d or st[2] != 1 or x.dtype != dtype
+            or (dtype != torch.bfloat16 and dtype != torch.float16) or x.get_device() != dev):
+        raise ValueError(f"{name} must be bf16 or fp16 [>= {n}, {hkv}, {d}] on cuda:{dev} with unit stride along the head dimension, got "
+                         f"{x.dtype} {tuple(shape)} strides {tuple(st)} on {x.device}")
+    return st[0], st[1]
 
 
 def kv_write(k: torch.Tensor, v: torch.Tensor, k_data: torch.Tensor, k_sf: torch.Tensor, v_data: torch.Tensor,
@@ -351,20 +377,18 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, k_data: torch.Tensor, k_sf: torch
     rows behind the last slot are not written.  Slots must be distinct.  Pool tensors as for ``resattn_decode``, head_dim any
     multiple of 16.  The bytes are those of the NVFP4 quantisers with global scale ``1 / *_global_scale``."""
     pages, code_stride, sf_stride, hkv, d, page = _kv_pool_args(k_data, k_sf, v_data, v_sf)
-    dev = k_data.device
+    dev = k_data.get_device()
     bits = _check_slots(slots, dev)
-    n = slots.shape[0]
-    for name, x in (("k", k), ("v", v)):
-        if (x.dim() != 3 or x.shape[0] < n or x.shape[1] != hkv or x.shape[2] != d or x.dtype != k.dtype or x.device != dev
-                or x.dtype not in (torch.bfloat16, torch.float16) or x.stride(2) != 1):
-            raise ValueError(f"{name} must be bf16 or fp16 [>= {n}, {hkv}, {d}] on {dev} with unit stride along the head dimension, got "
-                             f"{x.dtype} {tuple(x.shape)} strides {tuple(x.stride())} on {x.device}")
-    with _on_device(dev):
+    n, dtype = slots.shape[0], k.dtype
+    k_token, k_head = _check_rows("k", k, n, hkv, d, dtype, dev)
+    v_token, v_head = _check_rows("v", v, n, hkv, d, dtype, dev)
+    with _on_device(k_data.device):
         st = _cabi.load().ri_kv_write_nvfp4(
-            k.data_ptr(), v.data_ptr(), _cabi.torch_dtype_code(k.dtype), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-            slots.data_ptr(), bits, n, k_data.data_ptr(), k_sf.data_ptr(), v_data.data_ptr(), v_sf.data_ptr(), pages,
-            code_stride, sf_stride, hkv, d, page, k_global_scale, v_global_scale, _cabi.current_stream(dev))
-    _cabi.check(st, "kv_write")
+            k.data_ptr(), v.data_ptr(), _cabi.DTYPE_BF16 if dtype == torch.bfloat16 else _cabi.DTYPE_FP16, k_token, k_head,
+            v_token, v_head, slots.data_ptr(), bits, n, k_data.data_ptr(), k_sf.data_ptr(), v_data.data_ptr(), v_sf.data_ptr(),
+            pages, code_stride, sf_stride, hkv, d, page, k_global_scale, v_global_scale, _cabi.raw_stream(dev))
+    if st:
+        _cabi.check(st, "kv_write")
 
 
 def kv_read(k_data: torch.Tensor, k_sf: torch.Tensor, v_data: torch.Tensor, v_sf: torch.Tensor, k_global_scale: float,
@@ -377,43 +401,45 @@ def kv_read(k_data: torch.Tensor, k_sf: torch.Tensor, v_data: torch.Tensor, v_sf
     ``cu_seqlens`` int32 [B + 1] and ``num_tokens`` rows: the sequences of the batch end to end.  Rows behind the last
     sequence stay as they are in a caller's ``out`` and are zero otherwise; tokens without a table entry are zero."""
     pages, code_stride, sf_stride, hkv, d, page = _kv_pool_args(k_data, k_sf, v_data, v_sf)
-    dev = k_data.device
-    bits, bt_stride, bt_cols, batch = 64, 0, 0, 0
+    dev = k_data.get_device()
+    bits, slots_ptr, bt_ptr, cu_ptr, bt_stride, bt_cols, batch = 64, None, None, None, 0, 0, 0
     if slots is not None:
         if block_tables is not None or cu_seqlens is not None:
             raise ValueError("give slots, or block_tables with cu_seqlens, not both")
         bits = _check_slots(slots, dev)
-        if num_tokens not in (None, slots.shape[0]):
-            raise ValueError(f"num_tokens {num_tokens} does not match {slots.shape[0]} slots")
-        n = slots.shape[0]
+        n, slots_ptr = slots.shape[0], slots.data_ptr()
+        if num_tokens is not None and num_tokens != n:
+            raise ValueError(f"num_tokens {num_tokens} does not match {n} slots")
     else:
         if block_tables is None or cu_seqlens is None or num_tokens is None:
             raise ValueError("give slots, or block_tables with cu_seqlens and num_tokens")
-        batch = block_tables.shape[0] if block_tables.dim() == 2 else 0
-        if (batch < 1 or block_tables.dtype != torch.int32 or block_tables.device != dev or block_tables.shape[1] < 1
+        shape = block_tables.shape
+        if (len(shape) != 2 or shape[0] < 1 or shape[1] < 1 or block_tables.dtype != torch.int32 or block_tables.get_device() != dev
                 or block_tables.stride(1) != 1):
-            raise ValueError(f"block_tables must be int32 [batch, max_pages_per_seq] on {dev} with unit column stride")
-        if cu_seqlens.dtype != torch.int32 or cu_seqlens.device != dev or tuple(cu_seqlens.shape) != (batch + 1,) or not cu_seqlens.is_contiguous():
-            raise ValueError(f"cu_seqlens must be contiguous int32 [{batch + 1}] on {dev}")
-        n, bt_stride, bt_cols = int(num_tokens), block_tables.stride(0), block_tables.shape[1]
+            raise ValueError(f"block_tables must be int32 [batch, max_pages_per_seq] on cuda:{dev} with unit column stride")
+        batch, bt_cols = shape
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.get_device() != dev or cu_seqlens.shape != (batch + 1,) or not cu_seqlens.is_contiguous():
+            raise ValueError(f"cu_seqlens must be contiguous int32 [{batch + 1}] on cuda:{dev}")
+        n, bt_stride, bt_ptr, cu_ptr = int(num_tokens), block_tables.stride(0), block_tables.data_ptr(), cu_seqlens.data_ptr()
         if n < 0:
             raise ValueError(f"num_tokens must not be negative, got {n}")
-    zero_tail = out is None
     if out is None:
-        k_out = torch.empty(n, hkv, d, dtype=dtype, device=dev)
-        v_out = torch.empty(n, hkv, d, dtype=dtype, device=dev)
+        k_out = torch.empty((n, hkv, d), dtype=dtype, device=k_data.device)
+        v_out = torch.empty_like(k_out)
     else:
         k_out, v_out = out
+        dtype = k_out.dtype
         for x in out:
-            if tuple(x.shape) != (n, hkv, d) or x.dtype != k_out.dtype or x.device != dev or not x.is_contiguous():
-                raise ValueError(f"out must be two contiguous [{n}, {hkv}, {d}] tensors of one type on {dev}")
-    with _on_device(dev):
+            if x.shape != (n, hkv, d) or x.dtype != dtype or x.get_device() != dev or not x.is_contiguous():
+                raise ValueError(f"out must be two contiguous [{n}, {hkv}, {d}] tensors of one type on cuda:{dev}")
+    with _on_device(k_data.device):
         st = _cabi.load().ri_kv_read_nvfp4(
             k_data.data_ptr(), k_sf.data_ptr(), v_data.data_ptr(), v_sf.data_ptr(), pages, code_stride, sf_stride, hkv, d, page,
-            _cabi.ptr(slots), bits, _cabi.ptr(block_tables), bt_stride, bt_cols, _cabi.ptr(cu_seqlens), batch, n,
-            k_global_scale, v_global_scale, k_out.data_ptr(), v_out.data_ptr(),
-            _cabi.torch_dtype_code(k_out.dtype, allow_f32=True), int(zero_tail), _cabi.current_stream(dev))
-    _cabi.check(st, "kv_read")
+            slots_ptr, bits, bt_ptr, bt_stride, bt_cols, cu_ptr, batch, n, k_global_scale, v_global_scale, k_out.data_ptr(),
+            v_out.data_ptr(), _cabi.DTYPE_BF16 if dtype == torch.bfloat16 else _cabi.torch_dtype_code(dtype, allow_f32=True),
+            out is None, _cabi.raw_stream(dev))
+    if st:
+        _cabi.check(st, "kv_read")
     return k_out, v_out
 
 
