@@ -258,9 +258,9 @@ def run_paged_fp4_decode_qmul4_tmem_nvfp4(q: torch.Tensor, pool: NvFp4PagedKVPoo
 
 
 def _check_pool(pool: NvFp4PagedKVPool) -> None:
-    want = (pool.num_kv_heads, pool.page_size, pool.head_dim // 2)
-    if tuple(pool.k_data.shape[1:]) != want:
-        raise ValueError(f"pool.k_data must be [pages, {want[0]}, {want[1]}, {want[2]}], got {tuple(pool.k_data.shape)}")
+    shape = pool.k_data.shape
+    if len(shape) != 4 or shape[1] != pool.num_kv_heads or shape[2] != pool.page_size or 2 * shape[3] != pool.head_dim:
+        raise ValueError(f"pool.k_data must be [pages, {pool.num_kv_heads}, {pool.page_size}, {pool.head_dim // 2}], got {tuple(shape)}")
 
 
 def write_paged_kv(key: torch.Tensor, value: torch.Tensor, pool: NvFp4PagedKVPool, slot_mapping: torch.Tensor) -> None:

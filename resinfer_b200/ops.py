@@ -304,23 +304,31 @@ def resattn_decode_shared_prefix(q: torch.Tensor, k_data: torch.Tensor, k_sf: to
         raise ValueError("seq_lens must be contiguous int32 [batch] on the Q device")
     if b and not 0 <= prefix_row < b:
         raise ValueError(f"prefix_row {prefix_row} is not a row of the block table ({b})")
-    lib, device = _cabi.load(), q.device
-    with _on_device(device):
-        if workspace is None:
-            need = lib.ri_resattn_shared_prefix_workspace_bytes(b, hq, d, prefix_splits, splits)
-            workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
-        elif workspace.dtype != torch.uint8 or workspace.get_device() != dev or not workspace.is_contiguous():
-            raise ValueError(f"workspace must be contiguous uint8 on cuda:{dev}")
-        bt, bt_stride = block_tables.data_ptr(), block_tables.stride(0)
-        st = lib.ri_resattn_decode_shared_prefix(
-            q.data_ptr(), k_data.data_ptr(), k_sf.data_ptr(), v_data.data_ptr(), v_sf.data_ptr(), pages, code_stride, sf_stride,
-            bt, bt_stride, bt_shape[1], bt + 4 * prefix_row * bt_stride, seq_lens.data_ptr(), prefix_len, b, hq, hkv, d, page,
-            max_kv_len, score_scale, out_scale, out.data_ptr(),
-            _cabi.DTYPE_BF16 if out.dtype == torch.bfloat16 else _cabi.torch_dtype_code(out.dtype, allow_f32=True), prefix_splits,
-            splits, workspace.data_ptr(), workspace.numel(), status_word(device).data_ptr(), _cabi.raw_stream(dev))
-    if st:
-        _cabi.check(st, "resattn_decode_shared_prefix")
+    if workspace is None:
+        need = _cabi.load().ri_resattn_shared_prefix_workspace_bytes(b, hq, d, prefix_splits, splits)
+        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+    elif workspace.dtype != torch.uint8 or workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous uint8 on cuda:{dev}")
+    bt, bt_stride = block_tables.data_ptr(), block_tables.stride(0)
+    _call(dev, "ri_resattn_decode_shared_prefix", (
+        q.data_ptr(), k_data.data_ptr(), k_sf.data_ptr(), v_data.data_ptr(), v_sf.data_ptr(), pages, code_stride, sf_stride, bt,
+        bt_stride, bt_shape[1], bt + 4 * prefix_row * bt_stride, seq_lens.data_ptr(), prefix_len, b, hq, hkv, d, page, max_kv_len,
+        score_scale, out_scale, out.data_ptr(),
+        _cabi.DTYPE_BF16 if out.dtype == torch.bfloat16 else _cabi.torch_dtype_code(out.dtype, allow_f32=True), prefix_splits,
+        splits, workspace.data_ptr(), workspace.numel(), status_word(q.device).data_ptr()))
     return out
+
+
+def _call(dev: int, name: str, args: tuple) -> None:
+    """A C-ABI call whose last argument is the stream, with the tensors' device current; raises on rejection."""
+    fn = getattr(_cabi.load(), name)
+    if torch._C._cuda_getDevice() == dev:
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if st:
+        _cabi.check(st, name)
 
 
 _BYTES = (torch.uint8, torch.int8, torch.float8_e4m3fn)
@@ -337,7 +345,7 @@ def _kv_pool_args(k_data: torch.Tensor, k_sf: torch.Tensor, v_data: torch.Tensor
         if (k_sf.shape == (pages, hkv, page, sf) and v_sf.shape == k_sf.shape and half % 8 == 0 and pages > 1
                 and cs[3] == 1 and cs[2] == half and cs[1] == page * half and cs[0] >= hkv * page * half
                 and ss[3] == 1 and ss[2] == sf and ss[1] == page * sf and ss[0] >= hkv * page * sf
-                and k_data.dtype in _BYTES and k_sf.dtype in _BYTES and v_data.dtype in _BYTES and v_sf.dtype in _BYTES):
+                and k_data.dtype == v_data.dtype == torch.uint8 and (k_sf.dtype == v_sf.dtype) and k_sf.dtype in _BYTES):
             return pages, cs[0], ss[0], hkv, half * 2, page
     if k_data.dim() != 4 or v_data.shape != k_data.shape or k_sf.dim() != 4 or v_sf.shape != k_sf.shape:
         raise ValueError(f"a paged NVFP4 pool is codes [pages, Hkv, page, D/2] and scales [pages, Hkv, page, D/16] for K and V, got "
@@ -382,13 +390,10 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, k_data: torch.Tensor, k_sf: torch
     n, dtype = slots.shape[0], k.dtype
     k_token, k_head = _check_rows("k", k, n, hkv, d, dtype, dev)
     v_token, v_head = _check_rows("v", v, n, hkv, d, dtype, dev)
-    with _on_device(k_data.device):
-        st = _cabi.load().ri_kv_write_nvfp4(
-            k.data_ptr(), v.data_ptr(), _cabi.DTYPE_BF16 if dtype == torch.bfloat16 else _cabi.DTYPE_FP16, k_token, k_head,
-            v_token, v_head, slots.data_ptr(), bits, n, k_data.data_ptr(), k_sf.data_ptr(), v_data.data_ptr(), v_sf.data_ptr(),
-            pages, code_stride, sf_stride, hkv, d, page, k_global_scale, v_global_scale, _cabi.raw_stream(dev))
-    if st:
-        _cabi.check(st, "kv_write")
+    _call(dev, "ri_kv_write_nvfp4", (
+        k.data_ptr(), v.data_ptr(), _cabi.DTYPE_BF16 if dtype == torch.bfloat16 else _cabi.DTYPE_FP16, k_token, k_head, v_token,
+        v_head, slots.data_ptr(), bits, n, k_data.data_ptr(), k_sf.data_ptr(), v_data.data_ptr(), v_sf.data_ptr(), pages,
+        code_stride, sf_stride, hkv, d, page, k_global_scale, v_global_scale))
 
 
 def kv_read(k_data: torch.Tensor, k_sf: torch.Tensor, v_data: torch.Tensor, v_sf: torch.Tensor, k_global_scale: float,
@@ -432,14 +437,11 @@ def kv_read(k_data: torch.Tensor, k_sf: torch.Tensor, v_data: torch.Tensor, v_sf
         for x in out:
             if x.shape != (n, hkv, d) or x.dtype != dtype or x.get_device() != dev or not x.is_contiguous():
                 raise ValueError(f"out must be two contiguous [{n}, {hkv}, {d}] tensors of one type on cuda:{dev}")
-    with _on_device(k_data.device):
-        st = _cabi.load().ri_kv_read_nvfp4(
-            k_data.data_ptr(), k_sf.data_ptr(), v_data.data_ptr(), v_sf.data_ptr(), pages, code_stride, sf_stride, hkv, d, page,
-            slots_ptr, bits, bt_ptr, bt_stride, bt_cols, cu_ptr, batch, n, k_global_scale, v_global_scale, k_out.data_ptr(),
-            v_out.data_ptr(), _cabi.DTYPE_BF16 if dtype == torch.bfloat16 else _cabi.torch_dtype_code(dtype, allow_f32=True),
-            out is None, _cabi.raw_stream(dev))
-    if st:
-        _cabi.check(st, "kv_read")
+    _call(dev, "ri_kv_read_nvfp4", (
+        k_data.data_ptr(), k_sf.data_ptr(), v_data.data_ptr(), v_sf.data_ptr(), pages, code_stride, sf_stride, hkv, d, page,
+        slots_ptr, bits, bt_ptr, bt_stride, bt_cols, cu_ptr, batch, n, k_global_scale, v_global_scale, k_out.data_ptr(),
+        v_out.data_ptr(), _cabi.DTYPE_BF16 if dtype == torch.bfloat16 else _cabi.torch_dtype_code(dtype, allow_f32=True),
+        out is None))
     return k_out, v_out
 
 
