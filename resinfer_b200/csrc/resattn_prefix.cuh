@@ -174,16 +174,36 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
   uint8_t* stage0 = smem + C::kOffStage;
   if (warp < C::kProdWarp) {
     // -------------------------------------------------------------- query prologue: NVFP4 and its NVFP4 residue
-    constexpr int kThr = C::kProdWarp * 32;
-    for (int i = threadIdx.x; i < C::kRows * C::kSfPerRow; i += kThr) {
-      const int r = i / C::kSfPerRow, blk = i % C::kSfPerRow, row = row0 + r;
-      BlockQ bq{};
-      if (row < rows) {
+    constexpr int kThr = C::kProdWarp * 32, kBlocks = C::kRows * C::kSfPerRow, kIt = (kBlocks + kThr - 1) / kThr;
+    uint4 x[kIt][2];                                           // a block of 16 values each; all loads in flight together
+#pragma unroll
+    for (int it = 0; it < kIt; ++it) {
+      const int i = threadIdx.x + it * kThr, row = row0 + i / C::kSfPerRow;
+      x[it][0] = x[it][1] = make_uint4(0, 0, 0, 0);
+      if (i < kBlocks && row < rows) {
         const int b = row / G, g = row - b * G;
-        float v[16];
-        load16(p.q + (int64_t(b) * p.hq + hkv * G + g) * D + blk * 16, v);
-        bq = quant_mext16(v, 1.0f, 1.0f);
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t(b) * p.hq + hkv * G + g) * D + (i % C::kSfPerRow) * 16);
+        x[it][0] = __ldg(src);
+        x[it][1] = __ldg(src + 1);
       }
+    }
+#pragma unroll 1
+    for (int it = 0; it < kIt; ++it) {
+      const int i = threadIdx.x + it * kThr;
+      if (i >= kBlocks) break;
+      const int r = i / C::kSfPerRow, blk = i % C::kSfPerRow;
+      uint4 lo = x[0][0], hi = x[0][1];
+#pragma unroll
+      for (int k = 1; k < kIt; ++k)
+        if (it == k) lo = x[k][0], hi = x[k][1];
+      const uint32_t u[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      float v[16];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        v[2 * k] = __uint_as_float(u[k] << 16);
+        v[2 * k + 1] = __uint_as_float(u[k] & 0xFFFF0000u);
+      }
+      const BlockQ bq = quant_mext16(v, 1.0f, 1.0f);
       const uint32_t off = swz_off<D>(r, blk * 8);
       *reinterpret_cast<uint2*>(smem + off) = bq.base;
       *reinterpret_cast<uint2*>(smem + C::kQBytes + off) = bq.res;

@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
       const uint8_t* st = ring + (k % C::kStages) * C::kStageBytes;
       const int t0 = (begin + warp + k * C::kWarps) * 16;
       // ---- scores of tokens t0 + i8 and t0 + i8 + 8
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
+      float sa[4][4] = {};                                             // four chains: base and residue, even and odd steps
 #pragma unroll
       for (int h = 0; h < C::kBlk; ++h) {                              // 32 values of the quarter at a time
         uint32_t ka[2][16];
@@ -175,15 +175,16 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
         }
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
-          mma_16816(s, ka[0][2 * ks], ka[1][2 * ks], ka[0][2 * ks + 1], ka[1][2 * ks + 1], qb[8 * h + ks][0], qb[8 * h + ks][1]);
-          mma_16816(s, ka[0][2 * ks], ka[1][2 * ks], ka[0][2 * ks + 1], ka[1][2 * ks + 1], qr[8 * h + ks][0], qr[8 * h + ks][1]);
+          mma_16816(sa[ks & 1], ka[0][2 * ks], ka[1][2 * ks], ka[0][2 * ks + 1], ka[1][2 * ks + 1], qb[8 * h + ks][0], qb[8 * h + ks][1]);
+          mma_16816(sa[2 + (ks & 1)], ka[0][2 * ks], ka[1][2 * ks], ka[0][2 * ks + 1], ka[1][2 * ks + 1], qr[8 * h + ks][0], qr[8 * h + ks][1]);
         }
       }
+      float s[4];
       const bool partial = t0 < p.kv_begin || t0 + 16 > L;             // some of the tokens are another's, or nobody's
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int tok = t0 + i8 + 8 * (u >> 1);
-        s[u] = partial && (tok < p.kv_begin || tok >= L) ? -INFINITY : s[u] * p.score_scale_log2;
+        s[u] = partial && (tok < p.kv_begin || tok >= L) ? -INFINITY : ((sa[0][u] + sa[1][u]) + (sa[2][u] + sa[3][u])) * p.score_scale_log2;
       }
       if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) > m[0] + kLazyThreshold || fmaxf(s[1], s[3]) > m[1] + kLazyThreshold)) {
 #pragma unroll
@@ -213,23 +214,33 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
 #pragma unroll
       for (int h = 0; h < C::kBlk; ++h) {
         const int blk = i8 + 8 * h;
+        uint32_t sp[2];                                                // (scale of token 2 q4, of 2 q4 + 1), (+ 8, + 9)
+        uint2 codes[4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int row = 2 * q4 + 8 * u;
+          uint32_t f0 = st[C::kOffVsf + row * C::kSfPerRow + blk], f1 = st[C::kOffVsf + (row + 1) * C::kSfPerRow + blk];
+          if (partial) {                                               // whatever lies there: 0 x P = 0
+            if (t0 + row < p.kv_begin || t0 + row >= L) f0 = 0;
+            if (t0 + row + 1 < p.kv_begin || t0 + row + 1 >= L) f1 = 0;
+          }
+          asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(sp[u]) : "r"(f0 | f1 << 8));
+          codes[2 * u] = *reinterpret_cast<const uint2*>(st + C::kOffV + row * C::kVPitch + blk * 8);
+          codes[2 * u + 1] = *reinterpret_cast<const uint2*>(st + C::kOffV + (row + 1) * C::kVPitch + blk * 8);
+        }
 #pragma unroll
         for (int w = 0; w < 2; ++w) {                                  // eight values of the block at a time
-          uint32_t va[4][4];
+          uint32_t ev[2][4], od[2][4];                                 // pairs of tokens: even values, odd values
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int row = 2 * q4 + (u & 1) + 8 * (u >> 1);
-            const uint32_t codes = *reinterpret_cast<const uint32_t*>(st + C::kOffV + row * C::kVPitch + blk * 8 + 4 * w);
-            uint32_t sf = st[C::kOffVsf + row * C::kSfPerRow + blk];
-            if (partial && (t0 + row < p.kv_begin || t0 + row >= L)) sf = 0;   // whatever lies there: 0 x P = 0
-            uint32_t s0, s1;
-            expand_scales(sf, s0, s1);
-            expand8(codes, bits_h2(s0), va[u]);
+          for (int u = 0; u < 2; ++u) {
+            // the two tokens' codes side by side in a byte, so that one conversion gives the operand's pair
+            const uint32_t c0 = w ? codes[2 * u].y : codes[2 * u].x, c1 = w ? codes[2 * u + 1].y : codes[2 * u + 1].x;
+            expand8((c0 & 0x0F0F0F0Fu) | ((c1 << 4) & 0xF0F0F0F0u), bits_h2(sp[u]), ev[u]);
+            expand8(((c0 >> 4) & 0x0F0F0F0Fu) | (c1 & 0xF0F0F0F0u), bits_h2(sp[u]), od[u]);
           }
 #pragma unroll
           for (int c = 0; c < 4; ++c)                                  // values 8 w + 2 c, + 1 of the block
-            mma_16816(o[8 * h + 4 * w + c], __byte_perm(va[0][c], va[1][c], 0x5410), __byte_perm(va[0][c], va[1][c], 0x7632),
-                      __byte_perm(va[2][c], va[3][c], 0x5410), __byte_perm(va[2][c], va[3][c], 0x7632), p0, p1);
+            mma_16816(o[8 * h + 4 * w + c], ev[0][c], od[0][c], ev[1][c], od[1][c], p0, p1);
         }
       }
       __syncwarp();                                                    // the stage may be refilled
