@@ -310,8 +310,9 @@ extern "C" int ri_resattn_decode_shared_prefix(
     if (code_page_stride == 0) code_page_stride = page_rows * (head_dim / 2);
     if (sf_page_stride == 0) sf_page_stride = page_rows * (head_dim / 16);
     RI_CHECK_ARG(code_page_stride >= page_rows * (head_dim / 2) && sf_page_stride >= page_rows * (head_dim / 16) &&
-                     code_page_stride % 16 == 0 && sf_page_stride % 16 == 0,
-                 "page strides (%lld, %lld bytes) must be multiples of 16 and hold a page's %lld rows",
+                     code_page_stride % 16 == 0 && sf_page_stride % 16 == 0 && code_page_stride < (int64_t(1) << 31) &&
+                     sf_page_stride < (int64_t(1) << 31),
+                 "page strides (%lld, %lld bytes) must be multiples of 16 below 2 GiB and hold a page's %lld rows",
                  (long long)code_page_stride, (long long)sf_page_stride, (long long)page_rows);
   }
   RI_CHECK_ARG(batch == 0 || (q_bf16 && k_data && k_sf && v_data && v_sf && block_tables && seq_lens && out && prefix_table),

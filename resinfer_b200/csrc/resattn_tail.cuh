@@ -76,8 +76,23 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
   const int G = p.group;
   // its inputs were complete when the launch in front released this one: only the merge waits for it
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int L = min(max(__ldg(p.seq_lens + b), 0), p.max_tokens);
   const int begin = p.kv_begin / 16 + split * p.groups_per_split;       // groups of 16 tokens, at their absolute places
+  // three loads that wait for nothing: the page of the warp's first group (if the row has it), a block of the query, the length
+  const int32_t* bt = p.block_tables + int64_t(b) * p.bt_stride;
+  auto page_at = [&](int group) -> int {
+    const int t0 = group * 16;
+    return t0 < p.max_tokens ? __ldg(bt + (p.page_shift >= 0 ? t0 >> p.page_shift : t0 / p.page_size)) : 0;
+  };
+  int page_next = page_at(begin + warp);
+  uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
+  const int qg = threadIdx.x / C::kSfPerRow, qblk = threadIdx.x % C::kSfPerRow;   // at most eight heads x kSfPerRow blocks: one per thread
+  static_assert(8 * C::kSfPerRow <= C::kThreads, "one block per thread");
+  if (qg < G) {
+    const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t(b) * p.hq + hkv * G + qg) * D + qblk * 16);
+    x0 = __ldg(src);
+    x1 = __ldg(src + 1);
+  }
+  const int L = min(max(__ldg(p.seq_lens + b), 0), p.max_tokens);
   const int end = L > p.kv_begin ? min(begin + p.groups_per_split, (L + 15) / 16) : begin;
   const int i8 = lane >> 2, q4 = lane & 3;
   float o[C::kMTiles][4];
@@ -87,29 +102,32 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
 
   if (begin < end) {                                                   // the whole CTA
     // ---------------------------------------------------------------- copies of the warp's first groups
-    const int32_t* bt = p.block_tables + int64_t(b) * p.bt_stride;
     uint8_t* ring = smem + warp * (C::kStages * C::kStageBytes);
     const int n = begin + warp < end ? (end - begin - warp + C::kWarps - 1) / C::kWarps : 0;   // groups of this warp
-    auto page_of = [&](int k) -> int {
-      const int t0 = (begin + warp + k * C::kWarps) * 16;
-      return k < n ? __ldg(bt + (p.page_shift >= 0 ? t0 >> p.page_shift : t0 / p.page_size)) : 0;
-    };
-    int page_next = page_of(0);
+    const uint8_t* const k_src = p.k_data + lane * 16;
+    const uint8_t* const v_src = p.v_data + lane * 16;
+    // lanes 0 .. kSfPerRow - 1 copy K's scales of a group, the next kSfPerRow V's
+    const uint8_t* const sf_src = (lane < C::kSfPerRow ? p.k_sf : p.v_sf) + (lane % C::kSfPerRow) * 16;
+    const uint32_t dst0 = smem_u32(ring) + lane * 16;
+    const uint32_t v_dst0 = smem_u32(ring) + C::kOffV + (lane / (C::kRowBytes / 16)) * C::kVPitch + (lane % (C::kRowBytes / 16)) * 16;
+    constexpr int kVStep = 32 / (C::kRowBytes / 16) * C::kVPitch;     // rows that 32 lanes cover
+    const uint32_t sf_dst0 = smem_u32(ring) + C::kOffKsf + lane * 16;  // V's scales follow K's
+    const int page_row0 = hkv * p.page_size, last_page = int(p.num_pages) - 1;
+    const int code_stride = int(p.code_page_stride), sf_stride = int(p.sf_page_stride);   // below 2 GiB: checked on the host
     auto fetch = [&](int k) {
       if (k < n) {
-        const int t0 = (begin + warp + k * C::kWarps) * 16;
-        const int64_t page = min(max(int64_t(page_next), int64_t(0)), p.num_pages - 1);
-        page_next = page_of(k + 1);
-        const int64_t row = int64_t(hkv) * p.page_size + (p.page_shift >= 0 ? (t0 & (p.page_size - 1)) : t0 % p.page_size);
-        const int64_t code = page * p.code_page_stride + row * C::kRowBytes, sf = page * p.sf_page_stride + row * C::kSfPerRow;
-        const uint32_t st = smem_u32(ring + (k % C::kStages) * C::kStageBytes);
+        const int group = begin + warp + k * C::kWarps, t0 = group * 16;
+        const int page = min(max(page_next, 0), last_page);
+        if (k + 1 < n) page_next = page_at(group + C::kWarps);
+        const int row = page_row0 + (p.page_shift >= 0 ? (t0 & (p.page_size - 1)) : t0 % p.page_size);
+        const int64_t code = int64_t(page) * code_stride + row * C::kRowBytes, sf = int64_t(page) * sf_stride + row * C::kSfPerRow;
+        const uint32_t st = (k % C::kStages) * C::kStageBytes;
 #pragma unroll
-        for (int c = lane; c < C::kRowBytes; c += 32) {                // 16 rows of kRowBytes / 16 chunks
-          cp_async16(st + c * 16, p.k_data + code + c * 16);
-          cp_async16(st + C::kOffV + (c / (C::kRowBytes / 16)) * C::kVPitch + (c % (C::kRowBytes / 16)) * 16, p.v_data + code + c * 16);
+        for (int c = 0; c < C::kRowBytes / 32; ++c) {                  // 16 rows of kRowBytes / 16 chunks
+          cp_async16(dst0 + st + c * 512, k_src + code + c * 512);
+          cp_async16(v_dst0 + st + c * kVStep, v_src + code + c * 512);
         }
-        if (lane < C::kSfPerRow) cp_async16(st + C::kOffKsf + lane * 16, p.k_sf + sf + lane * 16);
-        else if (lane < 2 * C::kSfPerRow) cp_async16(st + C::kOffVsf + (lane - C::kSfPerRow) * 16, p.v_sf + sf + (lane - C::kSfPerRow) * 16);
+        if (2 * C::kSfPerRow == 32 || lane < 2 * C::kSfPerRow) cp_async16(sf_dst0 + st, sf_src + sf);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -117,14 +135,16 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
     for (int k = 0; k < C::kStages - 1; ++k) fetch(k);
     // ---------------------------------------------------------------- query: NVFP4 and its residue, expanded to FP16
     __half* qs = reinterpret_cast<__half*>(smem + C::kOffQ);           // [base, residue][8 heads][D]
-    for (int i = threadIdx.x; i < 8 * C::kSfPerRow; i += C::kThreads) {
-      const int g = i / C::kSfPerRow, blk = i % C::kSfPerRow;
-      BlockQ bq{};
-      if (g < G) {
-        float v[16];
-        load16(p.q + (int64_t(b) * p.hq + hkv * G + g) * D + blk * 16, v);
-        bq = quant_mext16(v, 1.0f, 1.0f);
+    if (threadIdx.x < 8 * C::kSfPerRow) {                              // heads beyond the group: zeros
+      const uint32_t u[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+      float v[16];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        v[2 * k] = __uint_as_float(u[k] << 16);
+        v[2 * k + 1] = __uint_as_float(u[k] & 0xFFFF0000u);
       }
+      BlockQ bq{};
+      if (qg < G) bq = quant_mext16(v, 1.0f, 1.0f);
       uint32_t s0, s1;
       expand_scales(uint32_t(bq.sf) | uint32_t(bq.sf_res) << 8, s0, s1);
 #pragma unroll
@@ -134,7 +154,7 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
         uint32_t lo[4], hi[4];
         expand8(codes.x, s2, lo);
         expand8(codes.y, s2, hi);
-        uint4* dst = reinterpret_cast<uint4*>(qs + (part * 8 + g) * D + blk * 16);
+        uint4* dst = reinterpret_cast<uint4*>(qs + (part * 8 + qg) * D + qblk * 16);
         dst[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         dst[1] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       }
@@ -328,19 +348,36 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
   }
   // ---------------------------------------------------------------- merge: sixteen threads per head find the weights
   const int total = p.splits + p.prefix_splits - first;
-  float* w_sh = reinterpret_cast<float*>(smem + C::kOBytes);           // [total][8]: behind the warps' partials (kSmem is sized for it)
+  float* w_sh = reinterpret_cast<float*>(smem + C::kOBytes);           // [total][8] maxima, then weights; [total][8] row sums
+  float* l_sh = w_sh + total * 8;
+  constexpr int kBatch = 8 / kPer;                                     // partials whose loads are in flight together, per thread
+  float4 v[kPer][kBatch];
+  const float4* src0 = reinterpret_cast<const float4*>(p.o_part + (first * rows + row0) * D) + threadIdx.x;
+  auto load_batch = [&](int s0) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (s0 + j < total && threadIdx.x + k * C::kThreads < G * (D / 4))
+          v[k][j] = __ldcg(src0 + k * C::kThreads + (s0 + j) * rows * (D / 4));
+  };
+  load_batch(0);                                                       // before their weights are known
   {
     const int g = threadIdx.x >> 4, x16 = threadIdx.x & 15;
     float mm = head_m[g];
-    for (int s = x16; s < total && g < G; s += 16) mm = fmaxf(mm, __ldcg(p.m_part + (first + s) * rows + row0 + g));
+    for (int s = x16; s < total && g < G; s += 16) {
+      const float ms = __ldcg(p.m_part + (first + s) * rows + row0 + g), ls = __ldcg(p.l_part + (first + s) * rows + row0 + g);
+      w_sh[s * 8 + g] = ms;
+      l_sh[s * 8 + g] = ls;
+      mm = fmaxf(mm, ms);
+    }
 #pragma unroll
     for (int x = 8; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
     float ll = 0.f;
-    for (int s = x16; s < total && g < G; s += 16) {
-      const float ms = __ldcg(p.m_part + (first + s) * rows + row0 + g), ls = __ldcg(p.l_part + (first + s) * rows + row0 + g);
-      const float w = ms == -INFINITY ? 0.f : fast_exp2(ms - mm);
+    for (int s = x16; s < total && g < G; s += 16) {                   // this thread's own entries
+      const float ms = w_sh[s * 8 + g], w = ms == -INFINITY ? 0.f : fast_exp2(ms - mm);
       w_sh[s * 8 + g] = w;
-      if (w != 0.f) ll += w * ls;
+      if (w != 0.f) ll += w * l_sh[s * 8 + g];
     }
 #pragma unroll
     for (int x = 8; x > 0; x >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, x);
@@ -355,24 +392,29 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
-    const int c4 = threadIdx.x + k * C::kThreads, g = c4 / (D / 4);
-    if (g >= G) continue;
+    const int c4 = threadIdx.x + k * C::kThreads, g = min(c4 / (D / 4), 7);
     const float f = head_m[g];
-    float4 a = make_float4(f * acc[k].x, f * acc[k].y, f * acc[k].z, f * acc[k].w);
-    const float4* src = reinterpret_cast<const float4*>(p.o_part + (first * rows + row0) * D) + c4;
-    for (int s0 = 0; s0 < total; s0 += 8) {                            // eight loads in flight, added in order
-      float4 v[8];
-      float w[8];
+    acc[k].x *= f; acc[k].y *= f; acc[k].z *= f; acc[k].w *= f;
+  }
+  for (int s0 = 0; s0 < total; s0 += kBatch) {                         // in order
+    if (s0 > 0) load_batch(s0);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        w[j] = s0 + j < total ? w_sh[(s0 + j) * 8 + g] : 0.f;
-        v[j] = w[j] != 0.f ? __ldcg(src + (s0 + j) * rows * (D / 4)) : make_float4(0.f, 0.f, 0.f, 0.f);   // empty partials hold no data
-      }
+    for (int k = 0; k < kPer; ++k) {
+      const int c4 = threadIdx.x + k * C::kThreads, g = c4 / (D / 4);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        a.x += w[j] * v[j].x; a.y += w[j] * v[j].y; a.z += w[j] * v[j].z; a.w += w[j] * v[j].w;
+      for (int j = 0; j < kBatch; ++j) {
+        const float w = s0 + j < total && g < G ? w_sh[(s0 + j) * 8 + g] : 0.f;
+        if (w != 0.f) {                                                // empty partials hold no data
+          acc[k].x += w * v[k][j].x; acc[k].y += w * v[k][j].y; acc[k].z += w * v[k][j].z; acc[k].w += w * v[k][j].w;
+        }
       }
     }
+  }
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int c4 = threadIdx.x + k * C::kThreads, g = c4 / (D / 4);
+    if (g >= G) continue;
+    float4 a = acc[k];
     const float r = head_r[g];
     a.x *= r; a.y *= r; a.z *= r; a.w *= r;
     const int64_t oi = row0 * D + 4 * c4;
@@ -394,8 +436,8 @@ int launch_tail(const AttnParams& p, cudaStream_t st) {
   int dev = 0;
   RI_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) dev = 0;
-  const int weights = (p.splits + p.prefix_splits) * 8 * 4;
-  constexpr int kMost = C::kOBytes + 512 * 32 > C::kSmemBytes ? C::kOBytes + 512 * 32 : C::kSmemBytes;
+  const int weights = (p.splits + p.prefix_splits) * 8 * 4 * 2;
+  constexpr int kMost = C::kOBytes + 512 * 64 > C::kSmemBytes ? C::kOBytes + 512 * 64 : C::kSmemBytes;
   if (!attr_done[dev]) {
     RI_CUDA(cudaFuncSetAttribute(resattn_tail_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
     RI_CUDA(cudaFuncSetAttribute(resattn_tail_kernel<D>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
