@@ -131,19 +131,52 @@ def _cluster_splits(batch: int, heads: int, length: int, sms: int) -> int:
 @functools.lru_cache(maxsize=4096)
 def select_shared_prefix_plan(batch, num_kv_heads, group, prefix_len, max_kv_len, sm_count, *, head_dim=128):
     """(prefix_splits, splits) for a decode whose sequences share their first ``prefix_len`` tokens: the pieces of the
-    prefix (128 query rows of one KV head each; 0 = no launch of its own) and of the tokens behind it."""
+    prefix (128 query rows of one KV head each; 0 = no launch of its own) and of the tokens behind it.
+
+    The first launch takes one SM per CTA; the second's CTAs (``per_sm`` of them to an SM) read the sequences' own tokens on
+    the SMs that the first leaves free and wait there for its end.  So fewer, longer pieces of the prefix pay when the whole
+    second launch then fits beside it, and as many pieces as there are SMs when it does not.  Times in microseconds, fitted
+    on B200 within a tenth or so (32 sequences of 64 heads behind 8190 tokens, up to 1024 own: 4 pieces beside the second launch
+    30 us, 8 pieces in front of it 37 us; 64 sequences behind 32768, up to 2048 own: 104 us, in two pieces each)."""
     _check_output_dimension(head_dim, False)
-    steps = -(-prefix_len // (128 if head_dim == 128 else 64))
+    step, step_us, per_sm = (128, 0.9, 4) if head_dim == 128 else (64, 0.82, 2)
+    group_us = 0.24 if head_dim == 128 else 0.4               # 16 tokens of one KV head, by one of a CTA's four warps in turn
+    pairs = max(1, batch * num_kv_heads)
+    steps = -(-prefix_len // step)
     units = max(1, num_kv_heads * -(-(batch * group) // 128))
-    prefix_splits = 0
-    if steps:
-        piece = max(1, -(-steps // max(1, sm_count // units)))
-        prefix_splits = min(256, -(-steps // piece))
-    # the rest: four warps walk over a (sequence, KV head)'s tokens; pieces of 512 tokens or more, no more of them than run at once
-    rest = max(0, max_kv_len - (prefix_len // 16 * 16 if prefix_splits else 0))
-    slots = sm_count * (4 if head_dim == 128 else 2)
-    splits = max(1, min(-(-rest // 512), 2 * slots // max(1, batch * num_kv_heads), 64))
-    return prefix_splits, splits
+    rest = max(1, -(-(max_kv_len - prefix_len // 16 * 16) // 16))       # groups of 16 tokens of the longest sequence
+
+    def second(sms):                                          # (microseconds, pieces) of the second launch on so many SMs
+        best = None
+        for n in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64):
+            if n > 1 and (n - 1) * -(-rest // n) >= rest:
+                continue
+            longest = 5.0 + -(-rest // n) * group_us + (4.0 if n > 1 else 0.0)
+            load = pairs * (n * (5.0 + (4.0 if n > 1 else 0.0)) + rest * 0.5 * group_us) / (sms * per_sm)   # lengths average half the longest
+            t = max(longest, load) + (0.25 * longest if pairs * n > sms * per_sm else 0.0)
+            if best is None or t < best[0]:
+                best = (t, n)
+        return best
+
+    if steps == 0:
+        return 0, second(sm_count)[1]
+    best = None
+    for n in range(1, min(steps, 256, max(1, sm_count // units)) + 1):
+        if n > 1 and -(-steps // n) == -(-steps // (n - 1)):
+            continue                                          # no shorter pieces than with one fewer
+        waves = -(-units * n // sm_count)
+        first = waves * (7.0 + -(-steps // n) * step_us)
+        idle = sm_count - units * n
+        t, k = second(sm_count)
+        first += 0.15 * n                                     # every piece is one more partial to merge
+        total = first + t
+        if waves == 1 and idle > 0:
+            beside, m = second(idle)
+            if pairs * m <= idle * per_sm and max(first, beside) + 3.0 < total:
+                total, k = max(first, beside) + 3.0, m
+        if best is None or total < best[0]:
+            best = (total, n, k)
+    return best[1], best[2]
 
 
 def static_compile_plans(*, output_nvfp4=False, grouped_head_tile=16, residue_fold=True, head_dim=128):
