@@ -276,3 +276,61 @@ def test_refusals_on_the_device(cuda_device):
             call(**kw)
     empty = call(q=t["q"][:0], block_tables=t["block_tables"][:0], seq_lens=t["seq_lens"][:0], o=out[:0])
     assert empty.shape == (0, 16, 128)
+
+
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("rise,tokens", [(100.0, 2000), (120.0, 600), (-100.0, 2000), (0.0, 600)])
+def test_scores_that_grow_or_fall_along_the_prefix(cuda_device, device_rcp, d, rise, tokens):
+    """Every step raises every row's maximum (by up to 2^30 a step), or none does after the first.  A score of 120 in
+    log2 carries at most 120 * 2^-22 * 4 = 1.2e-4 from the FP32 products, within the bound's margin."""
+    from resinfer_b200.nvfp4.cute_attn import host
+    hkv, g, page, b = 1, 8, 32, 3
+    lens = [tokens + 40, tokens + 1, tokens]
+    pool = _pool(cuda_device, (tokens + 40) // page + 1, hkv, page, d, False)
+    gen = torch.Generator().manual_seed(3)
+    total = tokens + 40
+    ramp = torch.linspace(0, 1, total)[:, None, None] * (rise * np.log(2.0) / d ** 0.5)   # q = 1: score = sum over d / sqrt(d)
+    k = (ramp + 0.3 * torch.randn(total, hkv, d, generator=gen)).bfloat16().to(cuda_device)
+    v = torch.randn(total, hkv, d, generator=gen).bfloat16().to(cuda_device)
+    pool.k_global_scale, pool.v_global_scale = 0.004, 0.002
+    host.write_paged_kv(k, v, pool, torch.arange(total, device=cuda_device))
+    table = torch.arange(total // page + 1, dtype=torch.int32).repeat(b, 1)[:, :pool.k_data.shape[0]].contiguous()
+    kv = _as_numpy(pool, table, lens)
+    q = torch.ones(b, g * hkv, d) + 0.2 * torch.randn(b, g * hkv, d, generator=gen)
+    q = q.bfloat16()
+    t = {n: torch.from_numpy(kv[n]).to(cuda_device) for n in ("k_data", "k_sf", "v_data", "v_sf", "seq_lens")}
+    t["block_tables"], t["q"] = table.to(cuda_device), q.to(cuda_device)
+    want = reference(q.float().numpy(), kv, d ** -0.5, device_rcp)
+    for ps, sp in ((1, 1), (3, 2), (0, 1)):
+        got = run(t, kv, tokens, d ** -0.5, ps, sp)
+        for i in range(b):
+            assert rel_fro(got[i].cpu().numpy(), want[i]) < TOL_F32, (ps, sp, i)
+
+
+def test_a_query_that_is_not_finite_spoils_its_own_head_only(cuda_device):
+    kv, q, t = make(cuda_device, [400, 350, 300], 290, 2, 8, 128, 16)
+    clean = run(t, kv, 290, 0.1, 2, 2)
+    bad = t["q"].clone()
+    bad[1, 3], bad[2, 9, 5], bad[0, 15, 64] = float("nan"), float("inf"), float("-inf")
+    got = run(dict(t, q=bad), kv, 290, 0.1, 2, 2)
+    same = torch.ones(3, 16, dtype=torch.bool, device=cuda_device)
+    same[1, 3] = same[2, 9] = same[0, 15] = False
+    assert torch.equal(got[same], clean[same])
+
+
+@pytest.mark.parametrize("d,g", [(128, 8), (128, 4), (256, 6)])
+def test_zero_and_tiny_queries(cuda_device, device_rcp, d, g):
+    """Blocks of zeros, whole heads of zeros (a plain mean of V), and values whose block scale rounds to zero."""
+    lens, prefix = [400, 350, 0, 291], 290
+    kv, q, t = make(cuda_device, lens, prefix, 2, g, d, 32)
+    q[0, 1] = 0
+    q[1, 2, :16] = 0
+    q[1, 0, 16:48] = O.bf16_round(np.float32(1e-5))
+    q[3] = -0.0
+    t["q"].copy_(torch.from_numpy(q))
+    want = reference(q, kv, d ** -0.5, device_rcp)
+    for ps, sp in ((2, 2), (0, 1)):
+        got = run(t, kv, prefix, d ** -0.5, ps, sp)
+        for i in (0, 1, 3):
+            assert rel_fro(got[i].cpu().numpy(), want[i]) < TOL_F32, (ps, sp, i)
+        assert not got[2].any()
