@@ -304,7 +304,10 @@ int64_t ri_resattn_counter_bytes(int batch, int num_q_heads);
 /* ri_resattn_decode_strided for a batch whose sequences share their first prefix_len tokens (a system prompt, a document,
  * the prompt of many samples): those tokens are read and multiplied once for all sequences.  The reference refuses such
  * batches (quant/vllm_integration/attn/backend.py: "causal, non-cascade attention").  The result is that of
- * ri_resattn_decode_strided on the same block tables (q residue on, FP16 V and P whatever ri_resattn_set_pv_format says).
+ * ri_resattn_decode_strided on the same block tables (q residue on, FP16 V and P whatever ri_resattn_set_pv_format says),
+ * up to roundings: the query is NVFP4(q) + NVFP4(q - NVFP4(q)) with exact differences, where ri_resattn_decode* take them
+ * with an approximate reciprocal and settle differences that lie between two codes another way (2e-3 of the output).
+ * All prefix_len tokens of prefix_table must have been written, also where no sequence is that long.
  *   block_tables [batch, bt_stride] (bt_cols valid columns) cover every sequence from its first token; prefix_table is a
  *   row that holds the prefix's pages (usually block_tables itself, its first row).  A sequence no longer than the prefix
  *   attends to its own seq_lens[b] tokens of it; an empty one gives zeros.  The prefix may end inside a page (sequences

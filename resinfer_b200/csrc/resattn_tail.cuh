@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
         v[2 * k + 1] = __uint_as_float(u[k] & 0xFFFF0000u);
       }
       BlockQ bq{};
-      if (qg < G) bq = quant_mext16(v, 1.0f, 1.0f);
+      if (qg < G) bq = quant_query16(v);
       uint32_t s0, s1;
       expand_scales(uint32_t(bq.sf) | uint32_t(bq.sf_res) << 8, s0, s1);
 #pragma unroll

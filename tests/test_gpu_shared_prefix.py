@@ -22,6 +22,22 @@ def rel_fro(a, b):
     return float(np.linalg.norm(a - b) / max(np.linalg.norm(b), 1e-30))
 
 
+def scale_rcp(x):
+    """The reciprocal of a scale, and the scale itself for the reciprocal of one: what the definition divides by."""
+    y = 1.0 / np.asarray(x, np.float64)
+    grid = O.e4m3_decode(np.arange(1, 0x7F, dtype=np.uint8)).astype(np.float64)
+    near = grid[np.abs(grid[None] - y.reshape(-1, 1)).argmin(1)].reshape(y.shape)
+    return np.where(np.abs(y / near - 1) < 1e-6, near, y).astype(np.float32)
+
+
+def even(q):
+    """q with every block of 16 scaled so that its largest magnitude is 6 times a power of two."""
+    x = q.float().unflatten(-1, (-1, 16))
+    amax = x.abs().amax(-1, keepdim=True)
+    want = 6 * torch.exp2(torch.round(torch.log2(amax / 6)))
+    return torch.where(x.abs() == amax, torch.sign(x) * want, x * (want / amax) * 0.99).flatten(-2).to(q.dtype)
+
+
 def make(dev, lens, prefix, hkv, g, d, page, seed=1, heat=1.0):
     """A pool in which sequence b's first min(lens[b], prefix) tokens are shared pages (the page in which the prefix ends
     is copied).  numpy oracle inputs and device tensors."""
@@ -50,12 +66,12 @@ def make(dev, lens, prefix, hkv, g, d, page, seed=1, heat=1.0):
     return kv, q, t
 
 
-def reference(q, kv, sm, rcp):
-    """float64 [B, Hq, D] without output rounding; the query's codes with the device's reciprocals, as everywhere."""
+def reference(q, kv, sm):
+    """float64 [B, Hq, D] without output rounding."""
     b, hq, d = q.shape
     hkv, page = kv["k_data"].shape[1:3]
     g = hq // hkv
-    qb, qr = O.dequant_grouped_q(*O.nvfp4_quant_grouped_q(q.reshape(b, hkv, g, d), rcp=O.RecordingRcp(rcp)), g)
+    qb, qr = O.dequant_grouped_q(*O.nvfp4_quant_grouped_q(q.reshape(b, hkv, g, d), rcp=O.RecordingRcp(scale_rcp)), g)
     qq = qb.astype(np.float64) + qr
     kd, vd = O.dequant_paged(kv["k_data"], kv["k_sf"]), O.dequant_paged(kv["v_data"], kv["v_sf"])
     out = np.zeros((b, hkv, g, d))
@@ -103,11 +119,11 @@ CASES = [
 
 
 @pytest.mark.parametrize("lens,prefix,hkv,g,d,page,ps,splits,heat", CASES)
-def test_matches_definition(cuda_device, device_rcp, lens, prefix, hkv, g, d, page, ps, splits, heat):
+def test_matches_definition(cuda_device, lens, prefix, hkv, g, d, page, ps, splits, heat):
     from resinfer_b200 import ops
     kv, q, t = make(cuda_device, lens, prefix, hkv, g, d, page, heat=heat)
     sm = d ** -0.5
-    want = reference(q, kv, sm, device_rcp)
+    want = reference(q, kv, sm)
     got = run(t, kv, prefix, sm, ps, splits)
     assert torch.isfinite(got).all()
     assert rel_fro(got.cpu().numpy(), want) < TOL_F32
@@ -119,8 +135,9 @@ def test_matches_definition(cuda_device, device_rcp, lens, prefix, hkv, g, d, pa
     half = run(t, kv, prefix, sm, ps, splits, dtype=torch.bfloat16)
     assert torch.equal(half, got.to(torch.bfloat16))
     assert rel_fro(half.float().cpu().numpy(), want) < TOL_BF16
-    plain = torch.zeros_like(got)
+    assert torch.equal(run(t, kv, prefix, sm, ps, splits), got)   # no order that changes
+    t["q"] = even(t["q"])
+    got, plain = run(t, kv, prefix, sm, ps, splits), torch.zeros_like(got)
     ops.resattn_decode(t["q"], t["k_data"], t["k_sf"], t["v_data"], t["v_sf"], t["block_tables"].clamp(min=0), t["seq_lens"],
                        sm * kv["k_global_scale"], kv["v_global_scale"], plain, splits=2)
     assert rel_fro(got.cpu().numpy(), plain.cpu().numpy()) < 2 * TOL_F32
-    assert torch.equal(run(t, kv, prefix, sm, ps, splits), got)   # no order that changes

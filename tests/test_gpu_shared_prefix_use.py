@@ -2,14 +2,14 @@
 streams, in graphs, over interleaved pools and with whatever lies in memory that nobody has written.
 
 Tolerances are those of test_gpu_shared_prefix: 6e-4 in FP32, 3e-3 in BF16, twice the former between two FP32 results, and
-between two BF16 results the roundings of both on top (2 * 2.3e-3 + 1.2e-3 < 6e-3)."""
+between two BF16 results the roundings of both on top (2 * 2.3e-3 + 1.2e-3 < 6e-3); `even` queries beside the plain decode."""
 import numpy as np
 import pytest
 import torch
 
 import oracle as O
 from test_gpu_kv_cache import _pool
-from test_gpu_shared_prefix import TOL_BF16, TOL_F32, make, reference, rel_fro, run
+from test_gpu_shared_prefix import TOL_BF16, TOL_F32, even, make, reference, rel_fro, run
 
 pytestmark = pytest.mark.gpu
 
@@ -27,7 +27,7 @@ def _slots(table, page, seq, lo, hi):
 
 @pytest.mark.parametrize("d,hkv,g,page,prefix,packed,dtype", [
     (128, 2, 8, 16, 150, False, torch.bfloat16), (256, 1, 4, 32, 97, True, torch.float16), (128, 3, 6, 128, 256, True, torch.bfloat16)])
-def test_a_generation(cuda_device, device_rcp, d, hkv, g, page, prefix, packed, dtype):
+def test_a_generation(cuda_device, d, hkv, g, page, prefix, packed, dtype):
     """A prompt is written once, three sequences append to it token by token, each step decodes; at the end the contexts
     are gathered.  All bytes that were never written are NaN scales."""
     from resinfer_b200 import ops
@@ -66,7 +66,7 @@ def test_a_generation(cuda_device, device_rcp, d, hkv, g, page, prefix, packed, 
                                                 prefix_row=step % 3)
         torch.cuda.synchronize()
         ops.check_status(q.device)
-        want = reference(q.float().cpu().numpy(), _as_numpy(pool, table, lens), d ** -0.5, device_rcp)
+        want = reference(q.float().cpu().numpy(), _as_numpy(pool, table, lens), d ** -0.5)
         assert not out[3].any()
         for s in range(3):
             assert rel_fro(out[s].float().cpu().numpy(), want[s]) < TOL_BF16, (step, s)
@@ -85,7 +85,7 @@ def test_a_generation(cuda_device, device_rcp, d, hkv, g, page, prefix, packed, 
 
 
 @pytest.mark.parametrize("d,page", [(128, 16), (256, 64), (128, 128)])
-def test_bytes_nobody_wrote(cuda_device, device_rcp, d, page):
+def test_bytes_nobody_wrote(cuda_device, d, page):
     """NaN scales and any codes behind every sequence's end, and in all pages that no table names."""
     lens, prefix = [333, 0, 90, 500, 333, 334], 333
     kv, q, t = make(cuda_device, lens, prefix, 2, 6, d, page)
@@ -95,7 +95,7 @@ def test_bytes_nobody_wrote(cuda_device, device_rcp, d, page):
             used[kv["block_tables"][i, tok // page], tok % page] = True
     for tok in range(prefix):
         used[kv["block_tables"][3, tok // page], tok % page] = True
-    want = reference(q, kv, d ** -0.5, device_rcp)
+    want = reference(q, kv, d ** -0.5)
     dead = torch.from_numpy(~used).to(cuda_device)[:, None, :, None]
     for x, byte in ((t["k_data"], 0x77), (t["k_sf"], 0x7F), (t["v_data"], 0xF7), (t["v_sf"], 0xFF)):
         x.masked_fill_(dead, byte)
@@ -105,11 +105,11 @@ def test_bytes_nobody_wrote(cuda_device, device_rcp, d, page):
             assert (not got[i].any()) if n == 0 else rel_fro(got[i].cpu().numpy(), want[i]) < TOL_F32, (ps, sp, i)
 
 
-def test_prefix_row_and_entries_that_name_no_page(cuda_device, device_rcp):
+def test_prefix_row_and_entries_that_name_no_page(cuda_device):
     """Padding in row 0, the prefix in row 2; table entries behind a sequence's end may hold anything."""
     lens, prefix, d, page = [0, 400, 290, 261], 256, 128, 16
     kv, q, t = make(cuda_device, lens, prefix, 2, 4, d, page)
-    want = reference(q, kv, d ** -0.5, device_rcp)
+    want = reference(q, kv, d ** -0.5)
     t["block_tables"][0] = -7
     for i, n in enumerate(lens):
         t["block_tables"][i, (n + page - 1) // page:] = 2 ** 31 - 1
@@ -121,10 +121,10 @@ def test_prefix_row_and_entries_that_name_no_page(cuda_device, device_rcp):
 
 
 @pytest.mark.parametrize("ps,sp", [(256, 1), (1, 256), (256, 256), (40, 3)])
-def test_most_pieces(cuda_device, device_rcp, ps, sp):
+def test_most_pieces(cuda_device, ps, sp):
     """More pieces than there is work for: empty partials, and a merge of up to 512 of them."""
     kv, q, t = make(cuda_device, [6000, 5121, 5200], 5120, 1, 8, 128, 64)
-    want = reference(q, kv, 128 ** -0.5, device_rcp)
+    want = reference(q, kv, 128 ** -0.5)
     got = run(t, kv, 5120, 128 ** -0.5, ps, sp)
     assert rel_fro(got.cpu().numpy(), want) < TOL_F32
     assert torch.equal(run(t, kv, 5120, 128 ** -0.5, ps, sp), got)
@@ -144,6 +144,7 @@ def test_drawn_shapes_by_the_host_entry(cuda_device, seed):
     kv, q, t = make(cuda_device, lens, prefix, hkv, g, d, page, seed=seed, heat=float(rng.choice([0.5, 2.0])))
     pool = NvFp4PagedKVPool(hkv, d, t["k_data"], t["v_data"], t["k_sf"], t["v_sf"], page_size=page)
     sm, vs = d ** -0.5 * kv["k_global_scale"], kv["v_global_scale"]
+    t["q"] = even(t["q"])
     got, plain = torch.full_like(t["q"], float("nan")), torch.zeros_like(t["q"])
     host.run_paged_fp4_decode_shared_prefix(t["q"], pool, t["block_tables"], t["seq_lens"], prefix, sm, got, value_scale=vs, prefix_row=b - 1)
     ops.resattn_decode(t["q"], t["k_data"], t["k_sf"], t["v_data"], t["v_sf"], t["block_tables"].clamp(min=0), t["seq_lens"], sm, vs, plain, splits=4)
@@ -161,6 +162,7 @@ def test_many_short_sequences(cuda_device):
     from resinfer_b200 import ops
     n, prefix = 1500, 70
     kv, q, t = make(cuda_device, [prefix + 1 + i % 3 for i in range(n)], prefix, 1, 8, 128, 16)
+    t["q"] = even(t["q"])
     got = run(t, kv, prefix, 0.1, 1, 1)
     plain = torch.zeros_like(got)
     ops.resattn_decode(t["q"], t["k_data"], t["k_sf"], t["v_data"], t["v_sf"], t["block_tables"].clamp(min=0), t["seq_lens"],
@@ -168,7 +170,7 @@ def test_many_short_sequences(cuda_device):
     assert rel_fro(got.cpu().numpy(), plain.cpu().numpy()) < 2 * TOL_F32
 
 
-def test_pool_beyond_32_bit_offsets(cuda_device, device_rcp):
+def test_pool_beyond_32_bit_offsets(cuda_device):
     """Pages in the last megabytes of a pool of more than 4 GiB of codes."""
     from resinfer_b200 import ops
     lens, prefix, hkv, g, d, page = [300, 280], 256, 8, 4, 256, 128
@@ -280,7 +282,7 @@ def test_refusals_on_the_device(cuda_device):
 
 @pytest.mark.parametrize("d", [128, 256])
 @pytest.mark.parametrize("rise,tokens", [(100.0, 2000), (120.0, 600), (-100.0, 2000), (0.0, 600)])
-def test_scores_that_grow_or_fall_along_the_prefix(cuda_device, device_rcp, d, rise, tokens):
+def test_scores_that_grow_or_fall_along_the_prefix(cuda_device, d, rise, tokens):
     """Every step raises every row's maximum (by up to 2^30 a step), or none does after the first.  A score of 120 in
     log2 carries at most 120 * 2^-22 * 4 = 1.2e-4 from the FP32 products, within the bound's margin."""
     from resinfer_b200.nvfp4.cute_attn import host
@@ -300,7 +302,7 @@ def test_scores_that_grow_or_fall_along_the_prefix(cuda_device, device_rcp, d, r
     q = q.bfloat16()
     t = {n: torch.from_numpy(kv[n]).to(cuda_device) for n in ("k_data", "k_sf", "v_data", "v_sf", "seq_lens")}
     t["block_tables"], t["q"] = table.to(cuda_device), q.to(cuda_device)
-    want = reference(q.float().numpy(), kv, d ** -0.5, device_rcp)
+    want = reference(q.float().numpy(), kv, d ** -0.5)
     for ps, sp in ((1, 1), (3, 2), (0, 1)):
         got = run(t, kv, tokens, d ** -0.5, ps, sp)
         for i in range(b):
@@ -319,7 +321,7 @@ def test_a_query_that_is_not_finite_spoils_its_own_head_only(cuda_device):
 
 
 @pytest.mark.parametrize("d,g", [(128, 8), (128, 4), (256, 6)])
-def test_zero_and_tiny_queries(cuda_device, device_rcp, d, g):
+def test_zero_and_tiny_queries(cuda_device, d, g):
     """Blocks of zeros, whole heads of zeros (a plain mean of V), and values whose block scale rounds to zero."""
     lens, prefix = [400, 350, 0, 291], 290
     kv, q, t = make(cuda_device, lens, prefix, 2, g, d, 32)
@@ -328,7 +330,7 @@ def test_zero_and_tiny_queries(cuda_device, device_rcp, d, g):
     q[1, 0, 16:48] = O.bf16_round(np.float32(1e-5))
     q[3] = -0.0
     t["q"].copy_(torch.from_numpy(q))
-    want = reference(q, kv, d ** -0.5, device_rcp)
+    want = reference(q, kv, d ** -0.5)
     for ps, sp in ((2, 2), (0, 1)):
         got = run(t, kv, prefix, d ** -0.5, ps, sp)
         for i in (0, 1, 3):
