@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
   __shared__ float head_m[8], head_l[8], head_r[8];
   __shared__ int last_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = blockIdx.x, hkv = blockIdx.y, b = blockIdx.z;
+  const int hkv = blockIdx.x, b = blockIdx.y, split = blockIdx.z;   // pieces at the sequences' ends, often short, come last
   const int G = p.group;
   // its inputs were complete when the launch in front released this one: only the merge waits for it
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
       const int c4 = threadIdx.x + k * C::kThreads, g = c4 / (D / 4);
-      if (g < G) reinterpret_cast<float4*>(p.o_part + (split * rows + row0) * D)[c4] = acc[k];
+      if (g < G && begin < end) reinterpret_cast<float4*>(p.o_part + (split * rows + row0) * D)[c4] = acc[k];   // nobody reads an empty one's
       acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     if (threadIdx.x < G) {
@@ -444,7 +444,7 @@ int launch_tail(const AttnParams& p, cudaStream_t st) {
     attr_done[dev] = true;
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.splits, p.hkv, p.batch);
+  cfg.gridDim = dim3(p.hkv, p.batch, p.splits);
   cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = C::kOBytes + weights > C::kSmemBytes ? C::kOBytes + weights : C::kSmemBytes;
   cfg.stream = st;
