@@ -77,13 +77,15 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
   // its inputs were complete when the launch in front released this one: only the merge waits for it
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int begin = p.kv_begin / 16 + split * p.groups_per_split;       // groups of 16 tokens, at their absolute places
-  // three loads that wait for nothing: the page of the warp's first group (if the row has it), a block of the query, the length
+  // loads that wait for nothing: the pages of the warp's first groups (if the row has them), a block of the query, the length
   const int32_t* bt = p.block_tables + int64_t(b) * p.bt_stride;
   auto page_at = [&](int group) -> int {
     const int t0 = group * 16;
     return t0 < p.max_tokens ? __ldg(bt + (p.page_shift >= 0 ? t0 >> p.page_shift : t0 / p.page_size)) : 0;
   };
-  int page_next = page_at(begin + warp);
+  int pages[C::kStages];                                               // of the groups whose copies come first, and of the one behind them
+#pragma unroll
+  for (int k = 0; k < C::kStages; ++k) pages[k] = page_at(begin + warp + k * C::kWarps);
   uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
   const int qg = threadIdx.x / C::kSfPerRow, qblk = threadIdx.x % C::kSfPerRow;   // at most eight heads x kSfPerRow blocks: one per thread
   static_assert(8 * C::kSfPerRow <= C::kThreads, "one block per thread");
@@ -114,11 +116,10 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
     const uint32_t sf_dst0 = smem_u32(ring) + C::kOffKsf + lane * 16;  // V's scales follow K's
     const int page_row0 = hkv * p.page_size, last_page = int(p.num_pages) - 1;
     const int code_stride = int(p.code_page_stride), sf_stride = int(p.sf_page_stride);   // below 2 GiB: checked on the host
-    auto fetch = [&](int k) {
+    auto fetch = [&](int k, int page) {
       if (k < n) {
         const int group = begin + warp + k * C::kWarps, t0 = group * 16;
-        const int page = min(max(page_next, 0), last_page);
-        if (k + 1 < n) page_next = page_at(group + C::kWarps);
+        page = min(max(page, 0), last_page);
         const int row = page_row0 + (p.page_shift >= 0 ? (t0 & (p.page_size - 1)) : t0 % p.page_size);
         const int64_t code = int64_t(page) * code_stride + row * C::kRowBytes, sf = int64_t(page) * sf_stride + row * C::kSfPerRow;
         const uint32_t st = (k % C::kStages) * C::kStageBytes;
@@ -132,7 +133,8 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
-    for (int k = 0; k < C::kStages - 1; ++k) fetch(k);
+    for (int k = 0; k < C::kStages - 1; ++k) fetch(k, pages[k]);
+    int page_next = pages[C::kStages - 1];
     // ---------------------------------------------------------------- query: NVFP4 and its residue, expanded to FP16
     __half* qs = reinterpret_cast<__half*>(smem + C::kOffQ);           // [base, residue][8 heads][D]
     if (threadIdx.x < 8 * C::kSfPerRow) {                              // heads beyond the group: zeros
@@ -170,7 +172,8 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
       qr[ks][0] = vr.x; qr[ks][1] = vr.y;
     }
     for (int k = 0; k < n; ++k) {
-      fetch(k + C::kStages - 1);
+      fetch(k + C::kStages - 1, page_next);
+      if (k + C::kStages < n) page_next = page_at(begin + warp + (k + C::kStages) * C::kWarps);
       asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
       __syncwarp();
       const uint8_t* st = ring + (k % C::kStages) * C::kStageBytes;
