@@ -29,9 +29,15 @@ struct TlCfg {
   static constexpr int kOffV = 16 * kRowBytes, kOffKsf = kOffV + 16 * kVPitch, kOffVsf = kOffKsf + 16 * kSfPerRow;
   static constexpr int kStageBytes = kOffVsf + 16 * kSfPerRow;
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
-  static constexpr int kOBytes = kWarps * 8 * D * 4;           // the warps' partials, in the rings' place
-  static constexpr int kOffQ = kRingBytes > kOBytes ? kRingBytes : kOBytes;   // [2][8][D] FP16
-  static constexpr int kSmemBytes = kOffQ + 2 * 8 * D * 2;
+  // the warps' partials, in the rings' place: [8 heads][D / 16 blocks][16], pitches for which the sixteen 8-byte accesses of
+  // half a warp (four blocks, every other head) share a bank at most in pairs
+  static constexpr int kOBlock = 20, kOHead = D / 16 * kOBlock + 4;
+  static constexpr int kOBytes = kWarps * 8 * kOHead * 4;
+  // query [2][8 heads][4 quarters][D / 4] FP16: a pitch for which the accesses of half a warp (four heads, four quarters) do not
+  // share a bank.  Without the two pitches a CTA spent 1 us (head_dim 256: 2 us) on conflicts
+  static constexpr int kOffQ = kRingBytes > kOBytes ? kRingBytes : kOBytes;
+  static constexpr int kQQuarter = D / 4 + 4, kQHead = 4 * kQQuarter;
+  static constexpr int kSmemBytes = kOffQ + 2 * 8 * kQHead * 2;
   static constexpr int kKSteps = D / 16, kMTiles = D / 16, kBlk = D / 128;
 };
 
@@ -136,7 +142,7 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
     for (int k = 0; k < C::kStages - 1; ++k) fetch(k, pages[k]);
     int page_next = pages[C::kStages - 1];
     // ---------------------------------------------------------------- query: NVFP4 and its residue, expanded to FP16
-    __half* qs = reinterpret_cast<__half*>(smem + C::kOffQ);           // [base, residue][8 heads][D]
+    __half* qs = reinterpret_cast<__half*>(smem + C::kOffQ);
     if (threadIdx.x < 8 * C::kSfPerRow) {                              // heads beyond the group: zeros
       const uint32_t u[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
       float v[16];
@@ -156,9 +162,11 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
         uint32_t lo[4], hi[4];
         expand8(codes.x, s2, lo);
         expand8(codes.y, s2, hi);
-        uint4* dst = reinterpret_cast<uint4*>(qs + (part * 8 + qg) * D + qblk * 16);
-        dst[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        dst[1] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        uint2* dst = reinterpret_cast<uint2*>(qs + (part * 8 + qg) * C::kQHead + qblk / (D / 64) * C::kQQuarter + qblk % (D / 64) * 16);
+        dst[0] = make_uint2(lo[0], lo[1]);
+        dst[1] = make_uint2(lo[2], lo[3]);
+        dst[2] = make_uint2(hi[0], hi[1]);
+        dst[3] = make_uint2(hi[2], hi[3]);
       }
     }
     __syncthreads();
@@ -166,8 +174,8 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
     uint32_t qb[C::kKSteps][2], qr[C::kKSteps][2];
 #pragma unroll
     for (int ks = 0; ks < C::kKSteps; ++ks) {
-      const uint2 vb = *reinterpret_cast<const uint2*>(qs + i8 * D + q4 * (D / 4) + 4 * ks);
-      const uint2 vr = *reinterpret_cast<const uint2*>(qs + (8 + i8) * D + q4 * (D / 4) + 4 * ks);
+      const uint2 vb = *reinterpret_cast<const uint2*>(qs + i8 * C::kQHead + q4 * C::kQQuarter + 4 * ks);
+      const uint2 vr = *reinterpret_cast<const uint2*>(qs + (8 + i8) * C::kQHead + q4 * C::kQQuarter + 4 * ks);
       qb[ks][0] = vb.x; qb[ks][1] = vb.y;
       qr[ks][0] = vr.x; qr[ks][1] = vr.y;
     }
@@ -274,12 +282,12 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], x);
     __syncthreads();                                                   // every ring has been read
-    float* ow = reinterpret_cast<float*>(smem) + warp * 8 * D;         // [head][D]
+    float* ow = reinterpret_cast<float*>(smem) + warp * 8 * C::kOHead;
 #pragma unroll
     for (int t = 0; t < C::kMTiles; ++t) {
-      const int d = 16 * (i8 + 8 * (t / 8)) + 2 * (t % 8);
-      *reinterpret_cast<float2*>(ow + (2 * q4) * D + d) = make_float2(o[t][0], o[t][2]);
-      *reinterpret_cast<float2*>(ow + (2 * q4 + 1) * D + d) = make_float2(o[t][1], o[t][3]);
+      const int d = C::kOBlock * (i8 + 8 * (t / 8)) + 2 * (t % 8);
+      *reinterpret_cast<float2*>(ow + (2 * q4) * C::kOHead + d) = make_float2(o[t][0], o[t][2]);
+      *reinterpret_cast<float2*>(ow + (2 * q4 + 1) * C::kOHead + d) = make_float2(o[t][1], o[t][3]);
     }
   }
   if (lane < 4) {
@@ -307,13 +315,14 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
   float4 acc[kPer];
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
-    const int c4 = threadIdx.x + k * C::kThreads, g = c4 / (D / 4);
+    const int c4 = threadIdx.x + k * C::kThreads, g = c4 / (D / 4), c = c4 % (D / 4);
     acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (g < G && begin < end) {
+      const float* src = reinterpret_cast<const float*>(smem) + g * C::kOHead + c / 4 * C::kOBlock + c % 4 * 4;
 #pragma unroll
       for (int w = 0; w < C::kWarps; ++w) {
         const float f = warp_m[w][g];
-        const float4 v = reinterpret_cast<const float4*>(smem)[w * 2 * D + c4];
+        const float4 v = *reinterpret_cast<const float4*>(src + w * 8 * C::kOHead);
         acc[k].x += f * v.x; acc[k].y += f * v.y; acc[k].z += f * v.z; acc[k].w += f * v.w;
       }
     }
@@ -353,7 +362,7 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
   const int total = p.splits + p.prefix_splits - first;
   float* w_sh = reinterpret_cast<float*>(smem + C::kOBytes);           // [total][8] maxima, then weights; [total][8] row sums
   float* l_sh = w_sh + total * 8;
-  constexpr int kBatch = 8 / kPer;                                     // partials whose loads are in flight together, per thread
+  constexpr int kBatch = 8;                                            // partials whose loads are in flight together
   float4 v[kPer][kBatch];
   const float4* src0 = reinterpret_cast<const float4*>(p.o_part + (first * rows + row0) * D) + threadIdx.x;
   auto load_batch = [&](int s0) {
