@@ -413,12 +413,16 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
       const int c4 = threadIdx.x + k * C::kThreads, g = c4 / (D / 4);
+      float w[kBatch];
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const float w = s0 + j < total && g < G ? w_sh[(s0 + j) * 8 + g] : 0.f;
-        if (w != 0.f) {                                                // empty partials hold no data
-          acc[k].x += w * v[k][j].x; acc[k].y += w * v[k][j].y; acc[k].z += w * v[k][j].z; acc[k].w += w * v[k][j].w;
-        }
+      for (int j = 0; j < kBatch; ++j) w[j] = s0 + j < total && g < G ? w_sh[(s0 + j) * 8 + g] : 0.f;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {                               // no branches: 32 of them in a row took 1 us a batch
+        const bool some = w[j] != 0.f;                                 // empty partials hold no data
+        acc[k].x += w[j] * (some ? v[k][j].x : 0.f);
+        acc[k].y += w[j] * (some ? v[k][j].y : 0.f);
+        acc[k].z += w[j] * (some ? v[k][j].z : 0.f);
+        acc[k].w += w[j] * (some ? v[k][j].w : 0.f);
       }
     }
   }
