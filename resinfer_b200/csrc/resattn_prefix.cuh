@@ -124,23 +124,45 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // twice rounded reciprocal for the scale; here it is the scale itself, so that the residue is exact (a bf16 value minus
 // code x scale fits FP32) and one that lies on a border between two codes, which bf16 values do often, goes to the even
 // one.  Against attention over q + residues in 64 bits: 2.0e-3 with the reciprocal (single rows 2e-2), 2.5e-4 without.
+// (Products, differences and maxima in pairs: the prologue of 128 rows is bound by its instructions.)
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float absmax16(const float (&x)[16]) {
+  float a = max3(fabsf(x[0]), fabsf(x[1]), fabsf(x[2])), b = max3(fabsf(x[3]), fabsf(x[4]), fabsf(x[5]));
+  a = max3(a, fabsf(x[6]), fabsf(x[7]));
+  b = max3(b, fabsf(x[8]), fabsf(x[9]));
+  a = max3(a, fabsf(x[10]), fabsf(x[11]));
+  b = max3(b, fabsf(x[12]), fabsf(x[13]));
+  return max3(fmaxf(a, b), fabsf(x[14]), fabsf(x[15]));
+}
+__device__ __forceinline__ uint2 codes16(const float (&x)[16], float mult) {
+  const uint64_t m2 = pair64(__float_as_uint(mult), __float_as_uint(mult));
+  float lo[8], hi[8];
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    unpair64(mul2(pair64(__float_as_uint(x[i]), __float_as_uint(x[i + 1])), m2), lo[i], lo[i + 1]);
+    unpair64(mul2(pair64(__float_as_uint(x[8 + i]), __float_as_uint(x[9 + i])), m2), hi[i], hi[i + 1]);
+  }
+  return make_uint2(cvt_e2m1x8(lo), cvt_e2m1x8(hi));
+}
 __device__ __forceinline__ BlockQ quant_query16(const float (&x)[16]) {
   BlockQ q;
-  float amax = 0.f, r[16], hat[8];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i]));
-  q.base = quant_plain16(x, nvfp4_scale(amax, 1.0f, &q.sf));
+  q.base = codes16(x, nvfp4_scale(absmax16(x), 1.0f, &q.sf));
   const float s = decode_e4m3(q.sf);
-  e2m1x8_to_float(q.base.x, hat);
+  const uint64_t s2 = pair64(__float_as_uint(-s), __float_as_uint(-s));
+  float r[16], hat[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = residue_fma(x[i], hat[i], s);
-  e2m1x8_to_float(q.base.y, hat);
+  for (int h = 0; h < 2; ++h) {
+    e2m1x8_to_float(h ? q.base.y : q.base.x, hat);             // by shifts: see resattn_tail.cuh on unpacking bytes just packed
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r[8 + i] = residue_fma(x[8 + i], hat[i], s);
-  amax = 0.f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(r[i]));
-  q.res = quant_plain16(r, nvfp4_scale(amax, 1.0f, &q.sf_res));
+    for (int i = 0; i < 8; i += 2)
+      unpair64(fma2(pair64(__float_as_uint(hat[i]), __float_as_uint(hat[i + 1])), s2, pair64(__float_as_uint(x[8 * h + i]), __float_as_uint(x[8 * h + i + 1]))),
+               r[8 * h + i], r[8 * h + i + 1]);
+  }
+  q.res = codes16(r, nvfp4_scale(absmax16(r), 1.0f, &q.sf_res));
   return q;
 }
 
@@ -227,7 +249,8 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
         v[2 * k] = __uint_as_float(u[k] << 16);
         v[2 * k + 1] = __uint_as_float(u[k] & 0xFFFF0000u);
       }
-      const BlockQ bq = quant_query16(v);
+      BlockQ bq{};                                             // rows behind the batch: zero
+      if (row0 + r < rows) bq = quant_query16(v);
       const uint32_t off = swz_off<D>(r, blk * 8);
       *reinterpret_cast<uint2*>(smem + off) = bq.base;
       *reinterpret_cast<uint2*>(smem + C::kQBytes + off) = bq.res;

@@ -151,6 +151,8 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
         v[2 * k] = __uint_as_float(u[k] << 16);
         v[2 * k + 1] = __uint_as_float(u[k] & 0xFFFF0000u);
       }
+      // The branch is needed: where the bytes that cvt_e2m1x8 packs (mov.b32 w, {b0, b1, b2, b3}) reach expand8's unpacking
+      // (mov.b32 {b0, b1, b2, b3}, w) in a straight line, CUDA 12.9's compiler joins the two and the codes come out wrong
       BlockQ bq{};
       if (qg < G) bq = quant_query16(v);
       uint32_t s0, s1;
