@@ -11,13 +11,15 @@
 //   O^T[D x 8 heads]        += V^T . P^T                    V^T as the A operand: a thread holds a scale block of four tokens;
 //                                                           P^T comes from S^T's registers by a transposed 8 x 8 move
 //
-// The query is NVFP4 + NVFP4 residue as everywhere, both parts exact in FP16; P is rounded to FP16, all sums are FP32, a
-// maximum is raised when a score exceeds it by more than 2^8.
+// The query is NVFP4 + NVFP4 residue, both parts exact in FP16; P is rounded to FP16 (11 bits, the operand's), all sums are
+// FP32, a maximum is raised when a score exceeds it by more than 2^8.
 //
 // Eight rows and a few hundred tokens give the tensor cores' large tiles nothing to do: what counts is how soon a CTA
-// reads memory and how many run.  The decode kernel (21 warps, tensor memory, about 5 us from launch to merge) took 54 us
-// for 64 sequences of up to 2048 own tokens behind a prefix, whose 75 MB take 12; this form is bound by memory and by
-// the expansion's instructions.
+// reads memory and how many run.  What bounds it: instructions, 430 a group of 16 tokens and KV head, 140 of them the
+// expansion -- 340 MB of own tokens (256 sequences of up to 2048, 8 heads) 113 us = 3.0 TB/s at 59 % of the issue slots; and
+// 3 us before a CTA's first product and 2 behind its last -- 85 MB (64 sequences) 45 us, 24 MB (32 of up to 1024) 20.5 us.
+// The decode kernel's form (21 warps, tensor memory) in this place took 54 us for 75 MB; eight warps a CTA were slower
+// (340 MB: 136 us), more CTAs an SM spilled.
 //
 // Merge: the CTA adds its warps' partials (o, l, m) and, after waiting for the launch in front (griddepcontrol.wait), the
 // partials of the prefix's pieces; with several pieces per sequence the last one to finish does it (tickets).
