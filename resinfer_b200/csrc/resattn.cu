@@ -301,7 +301,7 @@ extern "C" int ri_resattn_decode_shared_prefix(
   RI_CHECK_ARG(prefix_len >= 0 && prefix_len <= cap, "the prefix (%d tokens) must lie within the block table (%lld)", prefix_len,
                (long long)cap);
   RI_CHECK_ARG(max_kv_len >= 0, "max_kv_len must be non-negative");
-  RI_CHECK_ARG(score_scale > 0.f && isfinite(score_scale) && isfinite(out_scale), "score_scale must be positive and finite, out_scale finite");
+  RI_CHECK_ARG(score_scale > 0.f && isfinite(score_scale * kLog2e) && isfinite(out_scale), "score_scale must be positive and finite, out_scale finite");
   RI_CHECK_ARG(splits >= 1 && splits <= 256 && prefix_splits >= 0 && prefix_splits <= 256, "splits must be in [1, 256], prefix splits in [0, 256]");
   const int64_t row_tiles = (int64_t(batch) * group + 127) / 128;
   RI_CHECK_ARG(row_tiles * num_kv_heads <= 65535, "%d sequences of %d heads are too many rows", batch, num_q_heads);

@@ -24,8 +24,9 @@
 // of two.  (Waiting for the other group's maximum first, or taking turns at the exponentials, cost more than it hid; so did a
 // polynomial in the place of an eighth, a quarter or half of the exponentials: 128 steps 121, 139, 146 us against 119.)
 // Measured: a step of 128 x 128 (head_dim 256: 128 x 64) 0.78 us with pages of 128 tokens, 1480 cycles, the special function
-// unit busy for 60 to 69 % and the tensor cores for 44 to 52 %; 1.17 us with pages of 16.  Before the first step 4 us (the query's
-// codes 2), behind the last 3.  64 sequences of 64 heads over 8 behind 32768 tokens, in four pieces: 59 us = 0.93 PFLOP/s, V in FP16.
+// unit busy for 60 % and the tensor cores for 44 to 51 %; 1.17 us with pages of 16.  Before the first step 4 us (the query's
+// codes 2), behind the last 3.  64 sequences of 64 heads over 8 behind 32768 tokens, in four pieces on 128 SMs: 57 us, 1.2
+// PFLOP/s of the two products.
 //
 // Roles (16 warps):
 //   0-3, 4-7   softmax, thread = row (tensor-memory lane); the first group takes the even steps, the second the odd ones
