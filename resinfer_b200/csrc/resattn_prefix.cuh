@@ -24,7 +24,7 @@
 // of two.  (Waiting for the other group's maximum first, or taking turns at the exponentials, cost more than it hid; so did a
 // polynomial in the place of an eighth, a quarter or half of the exponentials: 128 steps 121, 139, 146 us against 119.)
 // Measured: a step of 128 x 128 (head_dim 256: 128 x 64) 0.78 us with pages of 128 tokens, 1480 cycles, the special function
-// unit busy for 60 % and the tensor cores for 44 to 51 %; 1.17 us with pages of 16.  Before the first step 4 us (the query's
+// unit busy for 60 % and the tensor cores for 44 to 51 %; 0.87 us with pages of 16.  Before the first step 4 us (the query's
 // codes 2), behind the last 3.  64 sequences of 64 heads over 8 behind 32768 tokens, in four pieces on 128 SMs: 57 us, 1.2
 // PFLOP/s of the two products.
 //
@@ -33,8 +33,8 @@
 //   8-11       V conversion: codes x scales -> FP16 in the 128-byte-swizzled N-major operand layout
 //   12, 13     one thread each issues the scores' and the P.V products; warp 12 lays K's scales out for them
 //   14, 15     copies of codes (tiled TMA in the operand swizzle) and of scales (bulk), one lane per run of tokens that lie
-//              together in a page.  A small copy costs its issuer about 50 cycles: with pages of 16 tokens one warp for all
-//              32 copies of a step took 1.8 us a step.
+//              together in a page.  Small copies are what pages of 16 and 32 tokens cost: with V among them, all from one warp, a
+//              step took 1.8 us, from two warps 1.17; there the conversion warps load V themselves (0.87).
 // Every wait is bounded.  A role whose wait expires sets the abort flag, which ends all other waits at once, and runs on
 // through its loop (every address is in bounds whatever the data), so all roles meet at the end and the status word is set.
 template <int D>
@@ -171,7 +171,8 @@ __device__ __forceinline__ BlockQ quant_query16(const float (&x)[16]) {
   return q;
 }
 
-template <int D>
+// VDIRECT: the conversion warps load V's codes and scales from the pool into registers, a step ahead, instead of from the stages
+template <int D, bool VDIRECT>
 __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(const __grid_constant__ CUtensorMap k_map,
                                                                                   const __grid_constant__ CUtensorMap v_map,
                                                                                   const __grid_constant__ AttnParams p, int run) {
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(smem_u32(&bar_full[s]), 2);                    // codes, scales
-      mbar_init(smem_u32(&bar_empty[s]), C::kConv + 1);               // conversion warps + the commit of the scores' MMAs
+      mbar_init(smem_u32(&bar_empty[s]), VDIRECT ? 1 : C::kConv + 1); // conversion warps + the commit of the scores' MMAs
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(smem_u32(&bar_sfull[s]), 1);
@@ -428,31 +429,72 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
     // ============================================================ V conversion warps: 32 tokens x 64 head-dim values each
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     const int cw = warp - C::kFirstConv;
-    constexpr int kUnits = kStep / 32 * C::kDBlocks / C::kConv;   // 32 tokens x 64 values each
+    constexpr int kUnits = kStep / 32 * C::kDBlocks / C::kConv;   // 32 tokens x 64 values each, of the same tokens
+    static_assert(kUnits == 2 && C::kDBlocks % 2 == 0, "64 bytes of codes a thread");
+    const int tok = 32 * (cw * kUnits / C::kDBlocks) + lane, dblk0 = cw * kUnits % C::kDBlocks;
+    uint4 n0[kUnits], n1[kUnits];                              // VDIRECT: the next step's
+    uint2 nsf = make_uint2(0, 0);
+    int page_next = 0;
+    auto page_of = [&](int j) -> int {
+      const int t = (s_begin + j) * kStep + tok;
+      return j < steps && t < p.prefix_len ? __ldg(p.prefix_table + (p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size)) : 0;
+    };
+    auto load = [&](int j, int entry) {
+      const int t = (s_begin + j) * kStep + tok;
+      nsf = make_uint2(0, 0);
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) n0[u] = n1[u] = make_uint4(0, 0, 0, 0);
+      if (j < steps && t < p.prefix_len) {
+        const int64_t page = min(max(int64_t(entry), int64_t(0)), p.num_pages - 1);
+        const int row = hkv * p.page_size + (p.page_shift >= 0 ? (t & (p.page_size - 1)) : t % p.page_size);
+        const uint4* src = reinterpret_cast<const uint4*>(p.v_data + page * p.code_page_stride + int64_t(row) * C::kRowBytes + dblk0 * 32);
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+          n0[u] = __ldg(src + 2 * u);
+          n1[u] = __ldg(src + 2 * u + 1);
+        }
+        nsf = __ldg(reinterpret_cast<const uint2*>(p.v_sf + page * p.sf_page_stride + int64_t(row) * C::kSfPerRow + dblk0 * 4));
+      }
+    };
+    if constexpr (VDIRECT) {
+      load(0, page_of(0));
+      page_next = page_of(1);
+    }
     for (int j = 0, stg = 0, ph = 0; j < steps; ++j, stg = (stg + 1 == S ? 0 : stg + 1), ph ^= (stg == 0)) {
       const int vb = j & 1;
-      px_wait(smem_u32(&bar_full[stg]), ph, &abort_flag, 6);
-      const uint8_t* st = stage0 + stg * C::kStageBytes;
       uint4 c0[kUnits], c1[kUnits];
       uint32_t sfw[kUnits];
+      if constexpr (VDIRECT) {
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        const int unit = cw * kUnits + u, tok = 32 * (unit / C::kDBlocks) + lane, dblk = unit % C::kDBlocks;
-        c0[u] = c1[u] = make_uint4(0, 0, 0, 0);
-        sfw[u] = 0;
-        if ((s_begin + j) * kStep + tok < p.prefix_len) {
-          const uint8_t* src = st + C::kStgV;
-          c0[u] = *reinterpret_cast<const uint4*>(src + swz_off<D>(tok, 32 * dblk));
-          c1[u] = *reinterpret_cast<const uint4*>(src + swz_off<D>(tok, 32 * dblk + 16));
-          sfw[u] = *reinterpret_cast<const uint32_t*>(st + C::kStgVsf + tok * C::kSfPerRow + dblk * 4);
+        for (int u = 0; u < kUnits; ++u) {
+          c0[u] = n0[u];
+          c1[u] = n1[u];
+          sfw[u] = u ? nsf.y : nsf.x;
         }
+        load(j + 1, page_next);
+        page_next = page_of(j + 2);
+      } else {
+        px_wait(smem_u32(&bar_full[stg]), ph, &abort_flag, 6);
+        const uint8_t* st = stage0 + stg * C::kStageBytes;
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+          const int dblk = dblk0 + u;
+          c0[u] = c1[u] = make_uint4(0, 0, 0, 0);
+          sfw[u] = 0;
+          if ((s_begin + j) * kStep + tok < p.prefix_len) {
+            const uint8_t* src = st + C::kStgV;
+            c0[u] = *reinterpret_cast<const uint4*>(src + swz_off<D>(tok, 32 * dblk));
+            c1[u] = *reinterpret_cast<const uint4*>(src + swz_off<D>(tok, 32 * dblk + 16));
+            sfw[u] = *reinterpret_cast<const uint32_t*>(st + C::kStgVsf + tok * C::kSfPerRow + dblk * 4);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_empty[stg])); // the codes are in registers: the stage may be refilled
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_empty[stg]));   // the codes are in registers: the stage may be refilled
       if (j >= 2) px_wait(smem_u32(&bar_vfree[vb]), ((j >> 1) - 1) & 1, &abort_flag, 11);
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
-        const int unit = cw * kUnits + u, tok = 32 * (unit / C::kDBlocks) + lane, dblk = unit % C::kDBlocks;
+        const int dblk = dblk0 + u;
         const uint32_t words[8] = {c0[u].x, c0[u].y, c0[u].z, c0[u].w, c1[u].x, c1[u].y, c1[u].z, c1[u].w};
         uint32_t lo, hi, sc2[4];                               // the four block scales as FP16 pairs (s, s)
         asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
@@ -568,18 +610,18 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
         const uint32_t st = smem_u32(stage0 + stg * C::kStageBytes), full = smem_u32(&bar_full[stg]);
         if (lane == 0) {                                       // whole runs, also the one in which the prefix ends
           const int live = min(runs, (p.prefix_len - (s_begin + j) * kStep + run - 1) / run);
-          mbar_expect_tx(full, live * run * 2 * (codes ? C::kRowBytes : C::kSfPerRow));
+          mbar_expect_tx(full, live * run * (VDIRECT ? 1 : 2) * (codes ? C::kRowBytes : C::kSfPerRow));
         }
         __syncwarp();
         if (lane < runs && t0 < p.prefix_len) {
           const int row = lane * run;
           if (codes) {
             tma_load_3d(st + row * C::kRowBytes, &k_map, 0, in_row, int(page), full);
-            tma_load_3d(st + C::kStgV + row * C::kRowBytes, &v_map, 0, in_row, int(page), full);
+            if constexpr (!VDIRECT) tma_load_3d(st + C::kStgV + row * C::kRowBytes, &v_map, 0, in_row, int(page), full);
           } else {
             const int64_t sf = page * p.sf_page_stride + int64_t(in_row) * C::kSfPerRow;
             bulk_load_1d(st + C::kStgKraw + row * C::kSfPerRow, p.k_sf + sf, run * C::kSfPerRow, full);
-            bulk_load_1d(st + C::kStgVsf + row * C::kSfPerRow, p.v_sf + sf, run * C::kSfPerRow, full);
+            if constexpr (!VDIRECT) bulk_load_1d(st + C::kStgVsf + row * C::kSfPerRow, p.v_sf + sf, run * C::kSfPerRow, full);
           }
         }
       }
@@ -596,20 +638,18 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
   }
 }
 
-template <int D>
-int launch_prefix(const AttnParams& p, int prefix_splits, cudaStream_t st) {
+template <int D, bool VDIRECT>
+int launch_prefix_form(const AttnParams& p, int prefix_splits, int run, cudaStream_t st) {
   using C = PxCfg<D>;
   static bool attr_done[64] = {};
   int dev = 0;
   RI_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) dev = 0;
   if (!attr_done[dev]) {
-    RI_CUDA(cudaFuncSetAttribute(resattn_prefix_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
-    RI_CUDA(cudaFuncSetAttribute(resattn_prefix_kernel<D>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
+    RI_CUDA(cudaFuncSetAttribute(resattn_prefix_kernel<D, VDIRECT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+    RI_CUDA(cudaFuncSetAttribute(resattn_prefix_kernel<D, VDIRECT>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
     attr_done[dev] = true;
   }
-  int run = 16;                                                // tokens that lie together: divides the page size and the step
-  while (run < C::kStep && p.page_size % (2 * run) == 0) run *= 2;
   CUtensorMap k_map{}, v_map{};
   const int64_t page_rows = int64_t(p.hkv) * p.page_size;
   int s = make_pool_map<D>(&k_map, p.k_data, p.num_pages, page_rows, p.code_page_stride, run);
@@ -626,5 +666,17 @@ int launch_prefix(const AttnParams& p, int prefix_splits, cudaStream_t st) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, resattn_prefix_kernel<D>, k_map, v_map, p, run), "shared-prefix attention launch");
+  return cuda_status(cudaLaunchKernelEx(&cfg, resattn_prefix_kernel<D, VDIRECT>, k_map, v_map, p, run), "shared-prefix attention launch");
+}
+
+// the first launch of a shared-prefix decode.  V by way of the stages, or directly, us for 128 steps of 512 rows: head_dim 128
+// pages of 16 166 / 132, of 32 140 / 130, of 64 125 / 129, of 128 118 / 129; head_dim 256 pages of 16 269 / 280, of 128 239 / 285.
+// A TMA copy of 16 or 32 rows takes 150 cycles whatever it holds, 32 of them a step.
+template <int D>
+int launch_prefix(const AttnParams& p, int prefix_splits, cudaStream_t st) {
+  int run = 16;                                                // tokens that lie together: divides the page size and the step
+  while (run < PxCfg<D>::kStep && p.page_size % (2 * run) == 0) run *= 2;
+  if constexpr (D == 128)
+    if (run <= 32) return launch_prefix_form<D, true>(p, prefix_splits, run, st);
+  return launch_prefix_form<D, false>(p, prefix_splits, run, st);
 }
