@@ -37,7 +37,7 @@ def _call(lib, *, q=4096, ptr=4096, pages=8, cs=0, ss=0, bt=4096, bt_cols=8, pt=
     (dict(pages=0), b"bad batch"), (dict(pages=1 << 31), b"bad batch"), (dict(bt_cols=0), b"bad batch"),
     (dict(bt_cols=1 << 28), b"too long"), (dict(prefix=-1), b"within the block table"), (dict(prefix=129), b"within the block table"),
     (dict(max_len=-1), b"non-negative"), (dict(scale=0.0), b"positive and finite"), (dict(scale=-0.1), b"positive and finite"),
-    (dict(scale=float("nan")), b"positive and finite"), (dict(scale=float("inf")), b"positive and finite"),
+    (dict(scale=3e38), b"positive and finite"), (dict(scale=float("nan")), b"positive and finite"), (dict(scale=float("inf")), b"positive and finite"),
     (dict(out_scale=float("nan")), b"finite"), (dict(sp=0), b"splits must be"), (dict(sp=257), b"splits must be"),
     (dict(ps=-1), b"splits must be"), (dict(ps=257), b"splits must be"), (dict(batch=65535, hq=64, hkv=8, bt_cols=8, d=256), b"workspace"),
     (dict(batch=65535, hq=8 * 200, hkv=200), b"too many rows"), (dict(cs=1000), b"page strides"), (dict(ss=24), b"page strides"),
