@@ -434,10 +434,25 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
     const int tok = 32 * (cw * kUnits / C::kDBlocks) + lane, dblk0 = cw * kUnits % C::kDBlocks;
     uint4 n0[kUnits], n1[kUnits];                              // VDIRECT: the next step's
     uint2 nsf = make_uint2(0, 0);
-    int page_next = 0;
+    int pages[3] = {};                                         // table entries of steps j + 1, j + 2, j + 3
     auto page_of = [&](int j) -> int {
       const int t = (s_begin + j) * kStep + tok;
       return j < steps && t < p.prefix_len ? __ldg(p.prefix_table + (p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size)) : 0;
+    };
+    auto row_of = [&](int j, int entry) -> int64_t {           // the token's row: page, and row of the page
+      const int t = (s_begin + j) * kStep + tok;
+      return min(max(int64_t(entry), int64_t(0)), p.num_pages - 1) << 32 |
+             uint32_t(hkv * p.page_size + (p.page_shift >= 0 ? (t & (p.page_size - 1)) : t % p.page_size));
+    };
+    auto codes_at = [&](int64_t row) { return p.v_data + (row >> 32) * p.code_page_stride + (row & 0xffffffff) * C::kRowBytes + dblk0 * 32; };
+    auto scales_at = [&](int64_t row) { return p.v_sf + (row >> 32) * p.sf_page_stride + (row & 0xffffffff) * C::kSfPerRow + dblk0 * 4; };
+    auto fetch_l2 = [&](int j, int entry) {                    // a step's latency does not cover the HBM's
+      if (j < steps && (s_begin + j) * kStep + tok < p.prefix_len) {
+        const int64_t row = row_of(j, entry);
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(codes_at(row)));
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(codes_at(row) + 32));
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(scales_at(row)));
+      }
     };
     auto load = [&](int j, int entry) {
       const int t = (s_begin + j) * kStep + tok;
@@ -445,20 +460,23 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) n0[u] = n1[u] = make_uint4(0, 0, 0, 0);
       if (j < steps && t < p.prefix_len) {
-        const int64_t page = min(max(int64_t(entry), int64_t(0)), p.num_pages - 1);
-        const int row = hkv * p.page_size + (p.page_shift >= 0 ? (t & (p.page_size - 1)) : t % p.page_size);
-        const uint4* src = reinterpret_cast<const uint4*>(p.v_data + page * p.code_page_stride + int64_t(row) * C::kRowBytes + dblk0 * 32);
+        const int64_t row = row_of(j, entry);
+        const uint4* src = reinterpret_cast<const uint4*>(codes_at(row));
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
           n0[u] = __ldg(src + 2 * u);
           n1[u] = __ldg(src + 2 * u + 1);
         }
-        nsf = __ldg(reinterpret_cast<const uint2*>(p.v_sf + page * p.sf_page_stride + int64_t(row) * C::kSfPerRow + dblk0 * 4));
+        nsf = __ldg(reinterpret_cast<const uint2*>(scales_at(row)));
       }
     };
     if constexpr (VDIRECT) {
-      load(0, page_of(0));
-      page_next = page_of(1);
+      const int first = page_of(0);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) pages[k] = page_of(k + 1);
+      load(0, first);
+      fetch_l2(1, pages[0]);
+      fetch_l2(2, pages[1]);
     }
     for (int j = 0, stg = 0, ph = 0; j < steps; ++j, stg = (stg + 1 == S ? 0 : stg + 1), ph ^= (stg == 0)) {
       const int vb = j & 1;
@@ -471,8 +489,11 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
           c1[u] = n1[u];
           sfw[u] = u ? nsf.y : nsf.x;
         }
-        load(j + 1, page_next);
-        page_next = page_of(j + 2);
+        load(j + 1, pages[0]);
+        fetch_l2(j + 3, pages[2]);
+        pages[0] = pages[1];
+        pages[1] = pages[2];
+        pages[2] = page_of(j + 4);
       } else {
         px_wait(smem_u32(&bar_full[stg]), ph, &abort_flag, 6);
         const uint8_t* st = stage0 + stg * C::kStageBytes;
