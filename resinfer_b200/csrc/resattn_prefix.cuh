@@ -690,9 +690,9 @@ int launch_prefix_form(const AttnParams& p, int prefix_splits, int run, cudaStre
   return cuda_status(cudaLaunchKernelEx(&cfg, resattn_prefix_kernel<D, VDIRECT>, k_map, v_map, p, run), "shared-prefix attention launch");
 }
 
-// the first launch of a shared-prefix decode.  V by way of the stages, or directly, us for 128 steps of 512 rows: head_dim 128
-// pages of 16 166 / 132, of 32 140 / 130, of 64 125 / 129, of 128 118 / 129; head_dim 256 pages of 16 269 / 280, of 128 239 / 285.
-// A TMA copy of 16 or 32 rows takes 150 cycles whatever it holds, 32 of them a step.
+// the first launch of a shared-prefix decode.  V by way of the stages, or directly, us for 512 rows and 16384 tokens in two
+// pieces, caches cold: head_dim 128 pages of 16 90 / 74, of 32 77 / 73, of 64 71.6 / 73.3, of 128 68 / 73; head_dim 256 pages
+// of 16 148 / 152, of 128 137 / 149.  A TMA copy of 16 or 32 rows takes 150 cycles whatever it holds, and V is half of them.
 template <int D>
 int launch_prefix(const AttnParams& p, int prefix_splits, cudaStream_t st) {
   int run = 16;                                                // tokens that lie together: divides the page size and the step
