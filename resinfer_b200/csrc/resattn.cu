@@ -297,7 +297,8 @@ extern "C" int ri_resattn_decode_shared_prefix(
   RI_CHECK_ARG(batch >= 0 && batch <= 65535 && num_pages > 0 && num_pages < (int64_t(1) << 31) && bt_cols >= 1 && bt_stride >= 0 && num_kv_heads <= 65535,
                "bad batch / page pool / block table");
   const int64_t cap = bt_cols * page_size;
-  RI_CHECK_ARG(cap < (int64_t(1) << 31) - 256, "a block table of %lld tokens is too long", (long long)cap);
+  // up to 256 pieces, each rounded up to 16 tokens and read ahead of by a few hundred: token numbers stay within 31 bits
+  RI_CHECK_ARG(cap < (int64_t(1) << 31) - 65536, "a block table of %lld tokens is too long", (long long)cap);
   RI_CHECK_ARG(prefix_len >= 0 && prefix_len <= cap, "the prefix (%d tokens) must lie within the block table (%lld)", prefix_len,
                (long long)cap);
   RI_CHECK_ARG(max_kv_len >= 0, "max_kv_len must be non-negative");

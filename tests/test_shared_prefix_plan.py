@@ -35,7 +35,7 @@ def _call(lib, *, q=4096, ptr=4096, pages=8, cs=0, ss=0, bt=4096, bt_cols=8, pt=
     (dict(hkv=0), b"divisible"), (dict(hq=15), b"divisible"), (dict(hq=4), b"GQA"), (dict(hq=10, hkv=2), b"GQA"),
     (dict(page=8), b"page size"), (dict(page=40), b"page size"), (dict(batch=-1), b"bad batch"), (dict(batch=65536), b"bad batch"),
     (dict(pages=0), b"bad batch"), (dict(pages=1 << 31), b"bad batch"), (dict(bt_cols=0), b"bad batch"),
-    (dict(bt_cols=1 << 28), b"too long"), (dict(prefix=-1), b"within the block table"), (dict(prefix=129), b"within the block table"),
+    (dict(bt_cols=1 << 28), b"too long"), (dict(bt_cols=(1 << 27) - 4000), b"too long"), (dict(prefix=-1), b"within the block table"), (dict(prefix=129), b"within the block table"),
     (dict(max_len=-1), b"non-negative"), (dict(scale=0.0), b"positive and finite"), (dict(scale=-0.1), b"positive and finite"),
     (dict(scale=3e38), b"positive and finite"), (dict(scale=float("nan")), b"positive and finite"), (dict(scale=float("inf")), b"positive and finite"),
     (dict(out_scale=float("nan")), b"finite"), (dict(sp=0), b"splits must be"), (dict(sp=257), b"splits must be"),
