@@ -136,8 +136,9 @@ def select_shared_prefix_plan(batch, num_kv_heads, group, prefix_len, max_kv_len
     The first launch takes one SM per CTA; the second's CTAs (``per_sm`` of them to an SM) read the sequences' own tokens on
     the SMs that the first leaves free and wait there for its end.  So fewer, longer pieces of the prefix pay when the whole
     second launch then fits beside it, and as many pieces as there are SMs when it does not.  Times in microseconds, fitted
-    on B200 within a tenth or so (32 sequences of 64 heads behind 8190 tokens, up to 1024 own: 4 pieces beside the second launch
-    30 us, 8 pieces in front of it 37 us; 64 sequences behind 32768, up to 2048 own: 104 us, in two pieces each)."""
+    on B200: of 28 drawn shapes 24 lie within a tenth of the best of some forty plans, all within a seventh (32 sequences of 64
+    heads behind 8190 tokens, up to 1024 own: 5 pieces beside the second launch 25 us; 64 behind 32768, up to 2048 own: 103 us
+    in 4 pieces and 2 of the rest, 112 in 4 and 1)."""
     _check_output_dimension(head_dim, False)
     step, step_us, per_sm = (128, 0.9, 4) if head_dim == 128 else (64, 0.82, 2)
     group_us = 0.24 if head_dim == 128 else 0.4               # 16 tokens of one KV head, by one of a CTA's four warps in turn
@@ -151,8 +152,9 @@ def select_shared_prefix_plan(batch, num_kv_heads, group, prefix_len, max_kv_len
         for n in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64):
             if n > 1 and (n - 1) * -(-rest // n) >= rest:
                 continue
-            longest = 5.0 + -(-rest // n) * group_us + (4.0 if n > 1 else 0.0)
-            load = pairs * (n * (5.0 + (4.0 if n > 1 else 0.0)) + rest * 0.5 * group_us) / (sms * per_sm)   # lengths average half the longest
+            crowd = min(1.0, max(0.0, 1.3 * (pairs * n / sms - 1.0) / (per_sm - 1)))   # a CTA with an SM to itself is faster
+            longest = 5.0 + -(-rest // n) * group_us * (0.65 + 0.35 * crowd) + (3.5 + 0.4 * n if n > 1 else 0.0)
+            load = pairs * (n * (5.0 + (3.5 if n > 1 else 0.0)) + rest * 0.5 * group_us) / (sms * per_sm)   # lengths average half the longest
             t = max(longest, load) + (0.25 * longest if pairs * n > sms * per_sm else 0.0)
             if best is None or t < best[0]:
                 best = (t, n)
