@@ -136,17 +136,23 @@ def select_shared_prefix_plan(batch, num_kv_heads, group, prefix_len, max_kv_len
     The first launch takes one SM per CTA; the second's CTAs (``per_sm`` of them to an SM) read the sequences' own tokens on
     the SMs that the first leaves free and wait there for its end.  So fewer, longer pieces of the prefix pay when the whole
     second launch then fits beside it, and as many pieces as there are SMs when it does not.  Times in microseconds, fitted
-    on B200: of 28 drawn shapes 24 lie within a tenth of the best of some forty plans, all within a seventh (32 sequences of 64
+    on B200: of 28 drawn shapes 24 lie within a tenth of the best of some forty plans, all within a sixth (32 sequences of 64
     heads behind 8190 tokens, up to 1024 own: 5 pieces beside the second launch 25 us; 64 behind 32768, up to 2048 own: 103 us
     in 4 pieces and 2 of the rest, 112 in 4 and 1)."""
     _check_output_dimension(head_dim, False)
-    step, step_us, per_sm = (128, 0.9, 4) if head_dim == 128 else (64, 0.82, 2)
-    group_us = 0.24 if head_dim == 128 else 0.4               # 16 tokens of one KV head, by one of a CTA's four warps in turn
-    pairs = max(1, batch * num_kv_heads)
-    steps = -(-prefix_len // step)
-    units = max(1, num_kv_heads * -(-(batch * group) // 128))
+    steps = -(-prefix_len // (128 if head_dim == 128 else 64))
     rest = max(1, -(-(max_kv_len - prefix_len // 16 * 16) // 16))       # groups of 16 tokens of the longest sequence
+    low = max(0, rest.bit_length() - 5)                       # five leading bits: not reckoned anew at each step of a generation
+    return _shared_prefix_plan(max(1, batch * num_kv_heads), max(1, num_kv_heads * -(-(batch * group) // 128)), steps,
+                               -(-rest >> low) << low, sm_count, head_dim)
 
+
+@functools.lru_cache(maxsize=4096)
+def _shared_prefix_plan(pairs, units, steps, rest, sm_count, head_dim):
+    step_us, per_sm = (0.9, 4) if head_dim == 128 else (0.82, 2)
+    group_us = 0.24 if head_dim == 128 else 0.4               # 16 tokens of one KV head, by one of a CTA's four warps in turn
+
+    @functools.lru_cache(maxsize=None)
     def second(sms):                                          # (microseconds, pieces) of the second launch on so many SMs
         best = None
         for n in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64):
@@ -172,7 +178,7 @@ def select_shared_prefix_plan(batch, num_kv_heads, group, prefix_len, max_kv_len
         t, k = second(sm_count)
         first += 0.15 * n                                     # every piece is one more partial to merge
         total = first + t
-        if waves == 1 and idle > 0:
+        if waves == 1 and idle > 0 and (best is None or first + 3.0 < best[0]):
             beside, m = second(idle)
             if pairs * m <= idle * per_sm and max(first, beside) + 3.0 < total:
                 total, k = max(first, beside) + 3.0, m
