@@ -124,11 +124,19 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// NaN if one of them is.  The maxima of partials are joined so: a partial's m is -inf where it attends to nothing and holds
+// no data, and NaN where it attends to scores of NaN alone, from which no maximum is found -- which has to reach the output
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 
 // A block of the query as NVFP4 and the NVFP4 of what that leaves, global scale 1.  quant_mext16 takes the residue with a
 // twice rounded reciprocal for the scale; here it is the scale itself, so that the residue is exact (a bf16 value minus
 // code x scale fits FP32) and one that lies on a border between two codes, which bf16 values do often, goes to the even
 // one.  Against attention over q + residues in 64 bits: 2.0e-3 with the reciprocal (single rows 2e-2), 2.5e-4 without.
+// A NaN does not count for the block's magnitude and 16 of them have scale zero, there as here.
 // (Products, differences and maxima in pairs: the prologue of 128 rows is bound by its instructions.)
 __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   uint64_t d;
@@ -141,7 +149,7 @@ __device__ __forceinline__ float absmax16(const float (&x)[16]) {
   b = max3(b, fabsf(x[8]), fabsf(x[9]));
   a = max3(a, fabsf(x[10]), fabsf(x[11]));
   b = max3(b, fabsf(x[12]), fabsf(x[13]));
-  return max3(fmaxf(a, b), fabsf(x[14]), fabsf(x[15]));
+  return max3(max3(a, b, 0.f), fabsf(x[14]), fabsf(x[15]));
 }
 __device__ __forceinline__ uint2 codes16(const float (&x)[16], float mult) {
   const uint64_t m2 = pair64(__float_as_uint(mult), __float_as_uint(mult));
@@ -285,6 +293,7 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
     const int lim_max = __reduce_max_sync(0xffffffffu, lim);
     const float scale = p.score_scale_log2;
     float m = -INFINITY, l = 0.f;                              // this group's: the row's maximum as it last knew it, its row sum
+    if (grp == 0) row_m[r] = -INFINITY;                        // steps in which no lane's maximum moves leave it so
     if (lim_max <= s_begin * kStep) {
       // none of these rows reaches the split's tokens: their P is zero throughout
       if (grp == 0) {
@@ -396,8 +405,9 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
     }
     // ---------------------------------------------------------------- the rows' partials: half of the columns per group
     if (steps > 0) px_wait(smem_u32(&bar_pvdone[(steps - 1) & 1]), ((steps - 1) >> 1) & 1, &abort_flag, 12);
-    const float m_end = steps > 0 && lim_max > s_begin * kStep ? row_m[r] : -INFINITY;   // ordered by the products in between
+    float m_end = steps > 0 && lim_max > s_begin * kStep ? row_m[r] : -INFINITY;   // ordered by the products in between
     l = m == -INFINITY ? 0.f : l * fast_exp2(m - m_end);
+    if (m_end == -INFINITY && steps > 0 && lim > s_begin * kStep) m_end = __int_as_float(0x7fffffff);   // see max_nan
     if (grp == 1) row_l[r] = l;
     asm volatile("bar.sync %0, 64;" ::"r"(9 + quarter) : "memory");
     if (__any_sync(0xffffffffu, row < rows)) {                 // whole warps: the loads from tensor memory are collective

@@ -282,9 +282,11 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], x);
+      if (n > 0 && m[h] == -INFINITY) m[h] = __int_as_float(0x7fffffff);   // a group has at least one token: see max_nan
+    }
     __syncthreads();                                                   // every ring has been read
     float* ow = reinterpret_cast<float*>(smem) + warp * 8 * C::kOHead;
 #pragma unroll
@@ -305,7 +307,7 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
   // ---------------------------------------------------------------- the CTA's partial: weights 2^(m_w - m) of its warps
   if (threadIdx.x < 8) {
     float mm = -INFINITY, ll = 0.f;
-    for (int w = 0; w < C::kWarps; ++w) mm = fmaxf(mm, warp_m[w][threadIdx.x]);
+    for (int w = 0; w < C::kWarps; ++w) mm = max_nan(mm, warp_m[w][threadIdx.x]);
     for (int w = 0; w < C::kWarps; ++w) {
       const float f = warp_m[w][threadIdx.x] == -INFINITY ? 0.f : fast_exp2(warp_m[w][threadIdx.x] - mm);
       warp_m[w][threadIdx.x] = f;
@@ -385,10 +387,10 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
       const float ms = __ldcg(p.m_part + (first + s) * rows + row0 + g), ls = __ldcg(p.l_part + (first + s) * rows + row0 + g);
       w_sh[s * 8 + g] = ms;
       l_sh[s * 8 + g] = ls;
-      mm = fmaxf(mm, ms);
+      mm = max_nan(mm, ms);
     }
 #pragma unroll
-    for (int x = 8; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
+    for (int x = 8; x > 0; x >>= 1) mm = max_nan(mm, __shfl_xor_sync(0xffffffffu, mm, x));
     float ll = 0.f;
     for (int s = x16; s < total && g < G; s += 16) {                   // this thread's own entries
       const float ms = w_sh[s * 8 + g], w = ms == -INFINITY ? 0.f : fast_exp2(ms - mm);
