@@ -307,7 +307,7 @@ int64_t ri_resattn_counter_bytes(int batch, int num_q_heads);
  * ri_resattn_decode_strided on the same block tables (q residue on, FP16 V and P whatever ri_resattn_set_pv_format says),
  * up to roundings: the query is NVFP4(q) + NVFP4(q - NVFP4(q)) with exact differences, where ri_resattn_decode* take them
  * with an approximate reciprocal and settle differences that lie between two codes another way (2e-3 of the output).
- * All prefix_len tokens of prefix_table must have been written, also where no sequence is that long.
+ * Tokens of the prefix that no sequence reaches need not have been written.
  * A NaN in the query counts as in the quantisers: not for its block's magnitude, 16 of them as zeros.  NaN block scales of K
  * give NaN in the rows of their KV head that attend to them; those of V inside the prefix also in rows that end before them.
  *   block_tables [batch, bt_stride] (bt_cols valid columns) cover every sequence from its first token; prefix_table is a

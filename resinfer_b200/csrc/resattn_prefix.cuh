@@ -14,7 +14,8 @@
 // only raised when a score exceeds it by more than 2^8, so o is rarely rescaled.  FP16 holds the code x block scale products
 // exactly and P with 11 bits.
 //
-// Rows shorter than the prefix are masked at their own length; rows beyond the batch have length zero.
+// Rows shorter than the prefix are masked at their own length; rows beyond the batch have length zero.  What no row of the
+// tile attends to may be unwritten: its scores are masked and its V is taken as zeros.
 //
 // What bounds it: the special function unit, 16 exponentials a cycle and SM -- 1024 cycles for 128 x 128 scores, against
 // 512 + 256 for the two products -- and, close behind, issue slots and the latencies of the chain scores -> P -> product.
@@ -232,6 +233,13 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
   }
   __syncthreads();                                             // the barriers exist: the copies may begin
   uint8_t* stage0 = smem + C::kOffStage;
+  int longest = 0;                                             // V conversion: of the lengths of the tile's sequences, two per lane
+  if (warp >= C::kFirstConv && warp < C::kQkWarp) {
+    static_assert(C::kRows / 4 + 1 <= 64, "groups of four heads and more");
+    const int b0 = row0 / G + lane, b_end = (min(row0 + C::kRows, rows) - 1) / G + 1;
+    if (b0 < b_end) longest = __ldg(p.seq_lens + b0);
+    if (b0 + 32 < b_end) longest = max(longest, __ldg(p.seq_lens + b0 + 32));
+  }
   if (warp < C::kProdWarp) {
     // -------------------------------------------------------------- query prologue: NVFP4 and its NVFP4 residue
     constexpr int kThr = C::kProdWarp * 32, kBlocks = C::kRows * C::kSfPerRow, kIt = (kBlocks + kThr - 1) / kThr;
@@ -442,12 +450,14 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
     constexpr int kUnits = kStep / 32 * C::kDBlocks / C::kConv;   // 32 tokens x 64 values each, of the same tokens
     static_assert(kUnits == 2 && C::kDBlocks % 2 == 0, "64 bytes of codes a thread");
     const int tok = 32 * (cw * kUnits / C::kDBlocks) + lane, dblk0 = cw * kUnits % C::kDBlocks;
+    // Tokens that none of the tile's rows attends to need not have been written: whatever lies there, V is 0 (0 x P = 0)
+    const int v_len = min(__reduce_max_sync(0xffffffffu, longest), p.prefix_len);
     uint4 n0[kUnits], n1[kUnits];                              // VDIRECT: the next step's
     uint2 nsf = make_uint2(0, 0);
     int pages[3] = {};                                         // table entries of steps j + 1, j + 2, j + 3
     auto page_of = [&](int j) -> int {
       const int t = (s_begin + j) * kStep + tok;
-      return j < steps && t < p.prefix_len ? __ldg(p.prefix_table + (p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size)) : 0;
+      return j < steps && t < v_len ? __ldg(p.prefix_table + (p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size)) : 0;
     };
     auto row_of = [&](int j, int entry) -> int64_t {           // the token's row: page, and row of the page
       const int t = (s_begin + j) * kStep + tok;
@@ -457,7 +467,7 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
     auto codes_at = [&](int64_t row) { return p.v_data + (row >> 32) * p.code_page_stride + (row & 0xffffffff) * C::kRowBytes + dblk0 * 32; };
     auto scales_at = [&](int64_t row) { return p.v_sf + (row >> 32) * p.sf_page_stride + (row & 0xffffffff) * C::kSfPerRow + dblk0 * 4; };
     auto fetch_l2 = [&](int j, int entry) {                    // a step's latency does not cover the HBM's
-      if (j < steps && (s_begin + j) * kStep + tok < p.prefix_len) {
+      if (j < steps && (s_begin + j) * kStep + tok < v_len) {
         const int64_t row = row_of(j, entry);
         asm volatile("prefetch.global.L2 [%0];" ::"l"(codes_at(row)));
         asm volatile("prefetch.global.L2 [%0];" ::"l"(codes_at(row) + 32));
@@ -469,7 +479,7 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
       nsf = make_uint2(0, 0);
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) n0[u] = n1[u] = make_uint4(0, 0, 0, 0);
-      if (j < steps && t < p.prefix_len) {
+      if (j < steps && t < v_len) {
         const int64_t row = row_of(j, entry);
         const uint4* src = reinterpret_cast<const uint4*>(codes_at(row));
 #pragma unroll
@@ -512,7 +522,7 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
           const int dblk = dblk0 + u;
           c0[u] = c1[u] = make_uint4(0, 0, 0, 0);
           sfw[u] = 0;
-          if ((s_begin + j) * kStep + tok < p.prefix_len) {
+          if ((s_begin + j) * kStep + tok < v_len) {
             const uint8_t* src = st + C::kStgV;
             c0[u] = *reinterpret_cast<const uint4*>(src + swz_off<D>(tok, 32 * dblk));
             c1[u] = *reinterpret_cast<const uint4*>(src + swz_off<D>(tok, 32 * dblk + 16));

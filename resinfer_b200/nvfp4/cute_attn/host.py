@@ -302,8 +302,8 @@ def run_paged_fp4_decode_shared_prefix(q: torch.Tensor, pool: NvFp4PagedKVPool, 
     prompt, a document, the prompt of many samples): the prefix is read and multiplied once for all of them.
 
     ``block_tables`` and ``seq_lens`` are the decode's own: whole sequences, prefix included; row ``prefix_row`` must hold
-    all pages of the prefix, written throughout (rows may be padding, of length 0, or end inside the prefix).  ``sm_scale`` includes the K
-    global scale, ``value_scale`` is the V global scale.  ``max_seq_len``: an upper bound of ``seq_lens`` (0: taken from the
+    all pages of the prefix, written as far as the longest sequence goes (rows may be padding, of length 0, or end inside the
+    prefix).  ``sm_scale`` includes the K global scale, ``value_scale`` is the V global scale.  ``max_seq_len``: an upper bound of ``seq_lens`` (0: taken from the
     device, which synchronises).  ``plan``: (pieces of the prefix, pieces of the rest), chosen here without it.  BF16
     output; V and P in FP16."""
     _check_pool(pool)
