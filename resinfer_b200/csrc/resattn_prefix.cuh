@@ -170,7 +170,7 @@ __device__ __forceinline__ BlockQ quant_query16(const float (&x)[16]) {
   float r[16], hat[8];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    e2m1x8_to_float(h ? q.base.y : q.base.x, hat);             // by shifts: see resattn_tail.cuh on unpacking bytes just packed
+    e2m1x8_to_float(h ? q.base.y : q.base.x, hat);             // by shifts: see expand8_packed in resattn_tail.cuh
 #pragma unroll
     for (int i = 0; i < 8; i += 2)
       unpair64(fma2(pair64(__float_as_uint(hat[i]), __float_as_uint(hat[i + 1])), s2, pair64(__float_as_uint(x[8 * h + i]), __float_as_uint(x[8 * h + i + 1]))),

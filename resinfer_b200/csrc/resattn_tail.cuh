@@ -64,6 +64,13 @@ __device__ __forceinline__ void expand8(uint32_t codes, __half2 s2, uint32_t (&o
   out[2] = h2_bits(__hmul2(bits_h2(h2), s2));
   out[3] = h2_bits(__hmul2(bits_h2(h3), s2));
 }
+// the same for codes that cvt_e2m1x8 has just packed, each byte taken out by a shift.  Where the bytes that it packs (mov.b32 w,
+// {b0, b1, b2, b3}) reach expand8's unpacking (mov.b32 {b0, b1, b2, b3}, w) in a straight line, CUDA 12.9's compiler joins the
+// two and the codes come out wrong: expand8 is for codes from memory only
+__device__ __forceinline__ void expand8_packed(uint32_t codes, __half2 s2, uint32_t (&out)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = h2_bits(__hmul2(e2m1x2_to_half2((codes >> (8 * i)) & 0xFFu), s2));
+}
 // two E4M3 bytes (low half of v) -> FP16 pairs (s0, s0), (s1, s1)
 __device__ __forceinline__ void expand_scales(uint32_t v, uint32_t& s0, uint32_t& s1) {
   uint32_t h;
@@ -145,7 +152,7 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
     int page_next = pages[C::kStages - 1];
     // ---------------------------------------------------------------- query: NVFP4 and its residue, expanded to FP16
     __half* qs = reinterpret_cast<__half*>(smem + C::kOffQ);
-    if (threadIdx.x < 8 * C::kSfPerRow) {                              // heads beyond the group: zeros
+    if (threadIdx.x < 8 * C::kSfPerRow) {                              // heads beyond the group: zeros, as loaded
       const uint32_t u[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
       float v[16];
 #pragma unroll
@@ -153,10 +160,7 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
         v[2 * k] = __uint_as_float(u[k] << 16);
         v[2 * k + 1] = __uint_as_float(u[k] & 0xFFFF0000u);
       }
-      // The branch is needed: where the bytes that cvt_e2m1x8 packs (mov.b32 w, {b0, b1, b2, b3}) reach expand8's unpacking
-      // (mov.b32 {b0, b1, b2, b3}, w) in a straight line, CUDA 12.9's compiler joins the two and the codes come out wrong
-      BlockQ bq{};
-      if (qg < G) bq = quant_query16(v);
+      const BlockQ bq = quant_query16(v);
       uint32_t s0, s1;
       expand_scales(uint32_t(bq.sf) | uint32_t(bq.sf_res) << 8, s0, s1);
 #pragma unroll
@@ -164,8 +168,8 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
         const uint2 codes = part ? bq.res : bq.base;
         const __half2 s2 = bits_h2(part ? s1 : s0);
         uint32_t lo[4], hi[4];
-        expand8(codes.x, s2, lo);
-        expand8(codes.y, s2, hi);
+        expand8_packed(codes.x, s2, lo);
+        expand8_packed(codes.y, s2, hi);
         uint2* dst = reinterpret_cast<uint2*>(qs + (part * 8 + qg) * C::kQHead + qblk / (D / 64) * C::kQQuarter + qblk % (D / 64) * 16);
         dst[0] = make_uint2(lo[0], lo[1]);
         dst[1] = make_uint2(lo[2], lo[3]);
