@@ -210,6 +210,15 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
   if (split == 0 && blockIdx.y == 0 && p.splits > 1)           // tickets of the launch behind this one
     for (int i = threadIdx.x; i < p.batch * p.hkv; i += blockDim.x) p.split_counter[i] = 0;
 
+  if (steps <= 0) {                                            // more pieces than steps: empty partials, and nothing is begun
+    const int row = row0 + threadIdx.x;
+    if (threadIdx.x < C::kRows && row < rows) {
+      const int64_t slot = (int64_t(p.splits + split) * p.batch + row / G) * p.hq + hkv * G + row % G;
+      p.l_part[slot] = 0.f;
+      p.m_part[slot] = -INFINITY;
+    }
+    return;
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(smem_u32(&bar_full[s]), 2);                    // codes, scales
@@ -412,10 +421,10 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
       }
     }
     // ---------------------------------------------------------------- the rows' partials: half of the columns per group
-    if (steps > 0) px_wait(smem_u32(&bar_pvdone[(steps - 1) & 1]), ((steps - 1) >> 1) & 1, &abort_flag, 12);
-    float m_end = steps > 0 && lim_max > s_begin * kStep ? row_m[r] : -INFINITY;   // ordered by the products in between
+    px_wait(smem_u32(&bar_pvdone[(steps - 1) & 1]), ((steps - 1) >> 1) & 1, &abort_flag, 12);
+    float m_end = lim_max > s_begin * kStep ? row_m[r] : -INFINITY;   // ordered by the products in between
     l = m == -INFINITY ? 0.f : l * fast_exp2(m - m_end);
-    if (m_end == -INFINITY && steps > 0 && lim > s_begin * kStep) m_end = __int_as_float(0x7fffffff);   // see max_nan
+    if (m_end == -INFINITY && lim > s_begin * kStep) m_end = __int_as_float(0x7fffffff);   // see max_nan
     if (grp == 1) row_l[r] = l;
     asm volatile("bar.sync %0, 64;" ::"r"(9 + quarter) : "memory");
     if (__any_sync(0xffffffffu, row < rows)) {                 // whole warps: the loads from tensor memory are collective
@@ -627,7 +636,7 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
           mma_commit(smem_u32(&bar_pvdone[vb]));
           mma_commit(smem_u32(&bar_vfree[vb]));
         }
-        if (steps > 0) px_wait(smem_u32(&bar_pvdone[(steps - 1) & 1]), ((steps - 1) >> 1) & 1, &abort_flag, 13);   // nothing is in flight any more
+        px_wait(smem_u32(&bar_pvdone[(steps - 1) & 1]), ((steps - 1) >> 1) & 1, &abort_flag, 13);   // nothing is in flight any more
       }
       __syncwarp();
     } else {
