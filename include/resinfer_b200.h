@@ -359,6 +359,11 @@ int ri_kv_read_nvfp4(const uint8_t* k_data, const uint8_t* k_sf, const uint8_t* 
                      float k_global_scale, float v_global_scale, void* k_out, void* v_out, int out_dtype,
                      int zero_tail, void* stream);
 
+/* Test helper: in calls of ri_resattn_decode_shared_prefix from here on, the wait of `role` (0 the scores' products, 1 the
+ * P.V products, 2 the copies of codes, 3 the copies of scales) in front of step `step` of the first launch's first CTA counts
+ * as run out: that CTA gives up in order and sets the status word.  Any other role: none (the default). */
+void ri_resattn_set_prefix_expiry(int role, int step);
+
 /* Test helper: out[i] = rcp.approx.ftz.f32(in[i]) on the device (the quantisers' reciprocal). */
 int ri_rcp_approx(const float* in, float* out, int n, void* stream);
 

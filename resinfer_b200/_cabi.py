@@ -64,6 +64,7 @@ SIGNATURES = {
                                _i, _i, _i, _f, _f, _vp]),
     "ri_kv_read_nvfp4": (_i, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i, _i, _i, _vp, _i, _vp, _i64, _i64, _vp, _i, _i64,
                               _f, _f, _vp, _vp, _i, _i, _vp]),
+    "ri_resattn_set_prefix_expiry": (None, [_i, _i]),
     "ri_rcp_approx": (_i, [_vp, _vp, _i, _vp]),
 }
 

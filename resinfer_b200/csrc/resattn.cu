@@ -56,6 +56,7 @@ struct AttnParams {
   int max_tokens;                          // what a block table row can hold
   int kv_begin;                            // first token of the second launch (the prefix's length, or 0)
   const int32_t* prefix_table;             // page table row that holds the prefix
+  int expire;                              // test: role * 2^26 + step whose wait counts as run out, -1 for none
 };
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
@@ -279,6 +280,11 @@ extern "C" int64_t ri_resattn_shared_prefix_workspace_bytes(int batch, int num_q
   return ri_resattn_counter_bytes(batch, num_q_heads) + rows * head_dim * 4 + 2 * rows * 4;
 }
 
+static int g_prefix_expire = -1;
+extern "C" void ri_resattn_set_prefix_expiry(int role, int step) {
+  g_prefix_expire = role >= 0 && role < 4 && step >= 0 && step < (1 << 26) ? (role << 26) + step : -1;
+}
+
 extern "C" int ri_resattn_decode_shared_prefix(
     const void* q_bf16, const uint8_t* k_data, const uint8_t* k_sf, const uint8_t* v_data, const uint8_t* v_sf,
     int64_t num_pages, int64_t code_page_stride, int64_t sf_page_stride, const int32_t* block_tables, int64_t bt_stride,
@@ -346,6 +352,7 @@ extern "C" int ri_resattn_decode_shared_prefix(
   p.prefix_len = prefix_len; p.prefix_splits = prefix_splits; p.prefix_table = prefix_table;
   p.kv_begin = prefix_splits > 0 ? prefix_len : 0;
   p.max_tokens = int(cap);
+  p.expire = g_prefix_expire;
   {
     const int step = head_dim == 128 ? tcattn::PxCfg<128>::kStep : tcattn::PxCfg<256>::kStep;
     const int64_t steps = (int64_t(prefix_len) + step - 1) / step;

@@ -36,8 +36,10 @@
 //   14, 15     copies of codes (tiled TMA in the operand swizzle) and of scales (bulk), one lane per run of tokens that lie
 //              together in a page.  Small copies are what pages of 16 and 32 tokens cost: with V among them, all from one warp, a
 //              step took 1.8 us, from two warps 1.17; there the conversion warps load V themselves (0.87).
-// Every wait is bounded.  A role whose wait expires sets the abort flag, which ends all other waits at once, and runs on
-// through its loop (every address is in bounds whatever the data), so all roles meet at the end and the status word is set.
+// Every wait is bounded.  A role whose wait expires sets the abort flag and leaves its loop, the others leave theirs at their
+// next wait that is not over, and none begins a copy or a product after that.  What is in flight then is waited for whatever
+// the flag says (px_drain): the products by a commit of their own, the copies by the barriers that count their bytes.  So all
+// roles meet at the end, nothing outlives the CTA, and the status word is set.
 template <int D>
 struct PxCfg {
   static constexpr int kStep = D == 128 ? 128 : 64;            // tokens per step
@@ -94,11 +96,35 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// A wait that returns when the phase is complete, or when the kernel has given up (see above).
-__device__ __forceinline__ void px_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int site) {
+// A wait that ends when the phase is complete (true), or when the kernel has given up (false, see above).  Short on purpose:
+// there are a dozen of them in loops that run side by side.  With mbar_wait inside, 64 sequences behind 32768 tokens took
+// 103.0 us instead of 101.1 before the roles looked at the results, and 106.6 instead of 102.4 since.
+__device__ __forceinline__ bool px_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int site) {
+  if (mbar_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_hint(bar, parity, 20000u)) {
+    if (*abort_flag) return false;
+    if (clock64() - t0 > kWaitLimitCycles) {
+      *abort_flag = site;                                      // which wait gave up (reported in the status word)
+      return false;
+    }
+  }
+  return true;
+}
+// ... for all lanes of a warp alike
+__device__ __forceinline__ bool px_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int site) {
+  return __all_sync(0xffffffffu, px_wait(bar, parity, abort_flag, site));
+}
+// A wait for what is in flight at the end, bounded, but not cut short by the abort flag.
+__device__ __forceinline__ void px_drain(uint32_t bar, uint32_t parity, volatile int* abort_flag, int site) {
   if (mbar_try(bar, parity)) return;
-  if (*abort_flag) return;
-  mbar_wait(bar, parity, abort_flag, site);
+  const long long t0 = clock64();
+  while (!mbar_try_hint(bar, parity, 20000u)) {
+    if (clock64() - t0 > kWaitLimitCycles) {
+      *abort_flag = site;
+      return;
+    }
+  }
 }
 
 // two FP32 operations per instruction; a pair is (low, high) of a 64-bit register
@@ -190,8 +216,10 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[S], bar_empty[S];
   __shared__ __align__(8) uint64_t bar_sfull[2], bar_sfree[2], bar_pready[2], bar_pvdone[2], bar_vready[2], bar_vfree[2];
+  __shared__ __align__(8) uint64_t bar_end[2];                 // all scores' products have ended, all P.V products
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
+  __shared__ volatile int copied[2];                           // steps whose codes (scales) have been asked for
   __shared__ float row_m[C::kRows], row_l[C::kRows];           // running maxima; row sums of the second group
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -231,6 +259,7 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
       mbar_init(smem_u32(&bar_pvdone[s]), 1);
       mbar_init(smem_u32(&bar_vready[s]), C::kConv);
       mbar_init(smem_u32(&bar_vfree[s]), 1);
+      mbar_init(smem_u32(&bar_end[s]), 1);
     }
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -242,6 +271,11 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
   }
   __syncthreads();                                             // the barriers exist: the copies may begin
   uint8_t* stage0 = smem + C::kOffStage;
+  // test: the first CTA's `role` gives up in front of a step
+  auto last_step = [&](int role) {
+    const int step = p.expire - (role << 26);
+    return step >= 0 && step < steps && blockIdx.x == 0 && blockIdx.y == 0 ? step : steps;
+  };
   int longest = 0;                                             // V conversion: of the lengths of the tile's sequences, two per lane
   if (warp >= C::kFirstConv && warp < C::kQkWarp) {
     static_assert(C::kRows / 4 + 1 <= 64, "groups of four heads and more");
@@ -323,9 +357,8 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
         tc_fence_before();
       }
       for (int j = grp, k = 0; j < steps; j += 2, ++k) {
-        px_wait(b_sfull, k & 1, &abort_flag, 5);
-        if (j > 0) px_wait(b_pvdone, ((j - 1) >> 1) & 1, &abort_flag, 7);
-        __syncwarp();
+        if (!px_wait_warp(b_sfull, k & 1, &abort_flag, 5)) break;
+        if (j > 0 && !px_wait_warp(b_pvdone, ((j - 1) >> 1) & 1, &abort_flag, 7)) break;
         if (lane == 0) {
           mbar_arrive(b_sfree);
           mbar_arrive(b_pready);
@@ -334,8 +367,7 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
     } else {
       for (int j = grp, k = 0; j < steps; j += 2, ++k) {
         const int left = lim - (s_begin + j) * kStep;          // of this row's tokens, from this step on
-        px_wait(b_sfull, k & 1, &abort_flag, 5);
-        __syncwarp();
+        if (!px_wait_warp(b_sfull, k & 1, &abort_flag, 5)) break;
         tc_fence_after();
         if (__any_sync(0xffffffffu, left < kStep)) {           // a row ends here: its scores beyond are -inf
 #pragma unroll 1
@@ -384,8 +416,7 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
         }
         float before = -INFINITY;
         if (j > 0) {                                           // P is free, the accumulator and row_m those of step j-1
-          px_wait(b_pvdone, ((j - 1) >> 1) & 1, &abort_flag, 7);
-          __syncwarp();
+          if (!px_wait_warp(b_pvdone, ((j - 1) >> 1) & 1, &abort_flag, 7)) break;
           tc_fence_after();
           before = row_m[r];
         }
@@ -524,7 +555,7 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
         pages[1] = pages[2];
         pages[2] = page_of(j + 4);
       } else {
-        px_wait(smem_u32(&bar_full[stg]), ph, &abort_flag, 6);
+        if (!px_wait_warp(smem_u32(&bar_full[stg]), ph, &abort_flag, 6)) break;
         const uint8_t* st = stage0 + stg * C::kStageBytes;
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
@@ -541,7 +572,7 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar_empty[stg])); // the codes are in registers: the stage may be refilled
       }
-      if (j >= 2) px_wait(smem_u32(&bar_vfree[vb]), ((j >> 1) - 1) & 1, &abort_flag, 11);
+      if (j >= 2 && !px_wait_warp(smem_u32(&bar_vfree[vb]), ((j >> 1) - 1) & 1, &abort_flag, 11)) break;
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         const int dblk = dblk0 + u;
@@ -585,9 +616,10 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
           tmem_cp_sf(sfq + 4 * i, desc_sf(smem_u32(smem) + C::kOffQsf + i * 512));
       }
       __syncwarp();
-      for (int j = 0, stg = 0, ph = 0; j < steps; ++j, stg = (stg + 1 == S ? 0 : stg + 1), ph ^= (stg == 0)) {
+      const int stop = last_step(0);
+      for (int j = 0, stg = 0, ph = 0; j < stop; ++j, stg = (stg + 1 == S ? 0 : stg + 1), ph ^= (stg == 0)) {
         const int sb = j & 1;
-        px_wait(smem_u32(&bar_full[stg]), ph, &abort_flag, 3);
+        if (!px_wait_warp(smem_u32(&bar_full[stg]), ph, &abort_flag, 3)) break;
         {                                                      // [token][group] -> [group of 64 values][32 rows][4 quarters] words
           uint8_t* st = stage0 + stg * C::kStageBytes;
 #pragma unroll
@@ -598,7 +630,7 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-        if (j >= 2) px_wait(smem_u32(&bar_sfree[sb]), ((j >> 1) - 1) & 1, &abort_flag, 4);
+        if (j >= 2 && !px_wait_warp(smem_u32(&bar_sfree[sb]), ((j >> 1) - 1) & 1, &abort_flag, 4)) break;
         tc_fence_after();
         __syncwarp();
         if (elect_one()) {
@@ -615,6 +647,12 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
         }
         __syncwarp();
       }
+      if (stop < steps) abort_flag = 3;
+      if (elect_one()) {
+        mma_commit(smem_u32(&bar_end[0]));
+        px_drain(smem_u32(&bar_end[0]), 0, &abort_flag, 17);
+      }
+      __syncwarp();
     } else if (warp == C::kPvWarp) {
       // ============================================================ P.V: a thread of another warp, so that the next scores do not
       // stand in line behind the exponentials
@@ -623,11 +661,12 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
       if (elect_one()) {
         // B = V: N-major, 128-byte swizzle: 64-d blocks 128 bytes x step apart (leading offset), 8-token groups 1 KB apart
         const uint64_t v_desc0 = desc_full(smem_u32(smem + C::kOffV), kStep * 128, 1024, 2);
-        for (int j = 0; j < steps; ++j) {
+        const int stop = last_step(1);
+        for (int j = 0; j < stop; ++j) {
           const int vb = j & 1;
           const uint64_t v_desc = v_desc0 + uint64_t((vb * C::kVBytes) >> 4);
-          px_wait(smem_u32(&bar_vready[vb]), (j >> 1) & 1, &abort_flag, 8);
-          px_wait(smem_u32(&bar_pready[vb]), (j >> 1) & 1, &abort_flag, 9);
+          if (!px_wait(smem_u32(&bar_vready[vb]), (j >> 1) & 1, &abort_flag, 8) ||
+              !px_wait(smem_u32(&bar_pready[vb]), (j >> 1) & 1, &abort_flag, 9)) break;
           tc_fence_after();
 #pragma unroll
           for (int k16 = 0; k16 < kStep / 16; ++k16)
@@ -636,7 +675,9 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
           mma_commit(smem_u32(&bar_pvdone[vb]));
           mma_commit(smem_u32(&bar_vfree[vb]));
         }
-        px_wait(smem_u32(&bar_pvdone[(steps - 1) & 1]), ((steps - 1) >> 1) & 1, &abort_flag, 13);   // nothing is in flight any more
+        if (stop < steps) abort_flag = 8;
+        mma_commit(smem_u32(&bar_end[1]));
+        px_drain(smem_u32(&bar_end[1]), 0, &abort_flag, 13);
       }
       __syncwarp();
     } else {
@@ -649,14 +690,14 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
         if (lane >= runs || j >= steps || t0 >= p.prefix_len) return 0;
         return __ldg(p.prefix_table + (p.page_shift >= 0 ? t0 >> p.page_shift : t0 / p.page_size));
       };
-      int page_next = lookup(0);
-      for (int j = 0, stg = 0, ph = 0; j < steps; ++j, stg = (stg + 1 == S ? 0 : stg + 1), ph ^= (stg == 0)) {
+      int page_next = lookup(0), armed = 0;
+      const int stop = last_step(codes ? 2 : 3);
+      for (int j = 0, stg = 0, ph = 0; j < stop; ++j, stg = (stg + 1 == S ? 0 : stg + 1), ph ^= (stg == 0)) {
         const int t0 = (s_begin + j) * kStep + lane * run;
         const int64_t page = min(max(int64_t(page_next), int64_t(0)), p.num_pages - 1);
         page_next = lookup(j + 1);
         const int in_row = hkv * p.page_size + (p.page_shift >= 0 ? (t0 & (p.page_size - 1)) : t0 % p.page_size);
-        if (j >= S) px_wait(smem_u32(&bar_empty[stg]), ph ^ 1, &abort_flag, 4);
-        __syncwarp();
+        if (j >= S && !px_wait_warp(smem_u32(&bar_empty[stg]), ph ^ 1, &abort_flag, 14)) break;
         const uint32_t st = smem_u32(stage0 + stg * C::kStageBytes), full = smem_u32(&bar_full[stg]);
         if (lane == 0) {                                       // whole runs, also the one in which the prefix ends
           const int live = min(runs, (p.prefix_len - (s_begin + j) * kStep + run - 1) / run);
@@ -674,9 +715,18 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
             if constexpr (!VDIRECT) bulk_load_1d(st + C::kStgVsf + row * C::kSfPerRow, p.v_sf + sf, run * C::kSfPerRow, full);
           }
         }
+        armed = j + 1;
       }
-      // nothing may be in flight when the CTA ends: the last stages' data have arrived
-      for (int j = max(steps - S, 0); j < steps; ++j) px_wait(smem_u32(&bar_full[j % S]), (j / S) & 1, &abort_flag, 15);
+      // The last stages' data have arrived before the CTA ends.  After a step that only one of the two warps has armed -- at
+      // most S of them, since a stage is refilled only when both have filled it, and none unless the kernel gives up -- the
+      // other arrives in its place, so that the phase counts the bytes to its end.
+      if (stop < steps) abort_flag = 14;
+      if (lane == 0) copied[codes ? 0 : 1] = armed;
+      asm volatile("bar.sync 14, 64;" ::: "memory");
+      const int most = max(armed, copied[codes ? 1 : 0]);
+      if (lane == 0)
+        for (int j = armed; j < most; ++j) mbar_arrive(smem_u32(&bar_full[j % S]));
+      for (int j = max(most - S, 0); j < most; ++j) px_drain(smem_u32(&bar_full[j % S]), (j / S) & 1, &abort_flag, 15);
     }
   }
   tc_fence_before();
