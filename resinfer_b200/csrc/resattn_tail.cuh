@@ -89,14 +89,16 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hkv = blockIdx.x, b = blockIdx.y, split = blockIdx.z;   // pieces at the sequences' ends, often short, come last
   const int G = p.group;
-  // its inputs were complete when the launch in front released this one: only the merge waits for it
+  // Its inputs were complete when the launch in front released this one: that launch waits for everything before it, and only
+  // then releases.  So only the merge waits for it here.  What this CTA reads before its own wait comes from the L2, where the
+  // writes of finished launches are (ld.global.cg, cp.async.cg): no line that an SM's L1 holds from before stands in for them.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int begin = p.kv_begin / 16 + split * p.groups_per_split;       // groups of 16 tokens, at their absolute places
   // loads that wait for nothing: the pages of the warp's first groups (if the row has them), a block of the query, the length
   const int32_t* bt = p.block_tables + int64_t(b) * p.bt_stride;
   auto page_at = [&](int group) -> int {
     const int t0 = group * 16;
-    return t0 < p.max_tokens ? __ldg(bt + (p.page_shift >= 0 ? t0 >> p.page_shift : t0 / p.page_size)) : 0;
+    return t0 < p.max_tokens ? __ldcg(bt + (p.page_shift >= 0 ? t0 >> p.page_shift : t0 / p.page_size)) : 0;
   };
   int pages[C::kStages];                                               // of the groups whose copies come first, and of the one behind them
 #pragma unroll
@@ -106,10 +108,10 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
   static_assert(8 * C::kSfPerRow <= C::kThreads, "one block per thread");
   if (qg < G) {
     const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t(b) * p.hq + hkv * G + qg) * D + qblk * 16);
-    x0 = __ldg(src);
-    x1 = __ldg(src + 1);
+    x0 = __ldcg(src);
+    x1 = __ldcg(src + 1);
   }
-  const int L = min(max(__ldg(p.seq_lens + b), 0), p.max_tokens);
+  const int L = min(max(__ldcg(p.seq_lens + b), 0), p.max_tokens);
   const int end = L > p.kv_begin ? min(begin + p.groups_per_split, (L + 15) / 16) : begin;
   const int i8 = lane >> 2, q4 = lane & 3;
   float o[C::kMTiles][4];
