@@ -754,8 +754,10 @@ int launch_prefix_form(const AttnParams& p, int prefix_splits, int run, cudaStre
   const int64_t page_rows = int64_t(p.hkv) * p.page_size;
   int s = make_pool_map<D>(&k_map, p.k_data, p.num_pages, page_rows, p.code_page_stride, run);
   if (s) return s;
-  s = make_pool_map<D>(&v_map, p.v_data, p.num_pages, page_rows, p.code_page_stride, run);
-  if (s) return s;
+  if constexpr (!VDIRECT) {
+    s = make_pool_map<D>(&v_map, p.v_data, p.num_pages, page_rows, p.code_page_stride, run);
+    if (s) return s;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(prefix_splits, p.hkv * ((p.batch * p.group + C::kRows - 1) / C::kRows));
   cfg.blockDim = dim3(C::kThreads);
