@@ -36,10 +36,10 @@
 //   14, 15     copies of codes (tiled TMA in the operand swizzle) and of scales (bulk), one lane per run of tokens that lie
 //              together in a page.  Small copies are what pages of 16 and 32 tokens cost: with V among them, all from one warp, a
 //              step took 1.8 us, from two warps 1.17; there the conversion warps load V themselves (0.87).
-// Every wait is bounded.  A role whose wait expires sets the abort flag and leaves its loop, the others leave theirs at their
-// next wait that is not over, and none begins a copy or a product after that.  What is in flight then is waited for whatever
-// the flag says (px_drain): the products by a commit of their own, the copies by the barriers that count their bytes.  So all
-// roles meet at the end, nothing outlives the CTA, and the status word is set.
+// Every wait is bounded.  A role whose wait expires sets the abort flag and leaves its loop (the scores': issues nothing more),
+// the others follow at their next wait that is not over, and none begins a copy or a product after that.  What is in flight
+// then is waited for whatever the flag says (px_drain): the products by a commit of their own, the copies by the barriers
+// that count their bytes.  So all roles meet at the end, nothing outlives the CTA, and the status word is set.
 template <int D>
 struct PxCfg {
   static constexpr int kStep = D == 128 ? 128 : 64;            // tokens per step
@@ -610,6 +610,9 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
       const uint64_t q_desc = desc_kmajor(smem_u32(smem), kSbo, kLayout);
       const uint64_t k_desc0 = desc_kmajor(smem_u32(stage0), kSbo, kLayout), ksf_desc0 = desc_sf(smem_u32(stage0) + C::kStgKsf);
       const uint32_t sfq = tmem_base + C::kColSfq;
+      // Each lane remembers its own waits, and the one that issues stops by what it saw: agreeing on it here, a step in the chain
+      // of the scores, cost 1 us of 64 steps
+      bool go = true;
       if (elect_one()) {
 #pragma unroll
         for (int i = 0; i < 2 * C::kMma; ++i)                  // the query scales, once
@@ -619,7 +622,7 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
       const int stop = last_step(0);
       for (int j = 0, stg = 0, ph = 0; j < stop; ++j, stg = (stg + 1 == S ? 0 : stg + 1), ph ^= (stg == 0)) {
         const int sb = j & 1;
-        if (!px_wait_warp(smem_u32(&bar_full[stg]), ph, &abort_flag, 3)) break;
+        go = go && px_wait(smem_u32(&bar_full[stg]), ph, &abort_flag, 3);
         {                                                      // [token][group] -> [group of 64 values][32 rows][4 quarters] words
           uint8_t* st = stage0 + stg * C::kStageBytes;
 #pragma unroll
@@ -630,10 +633,10 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-        if (j >= 2 && !px_wait_warp(smem_u32(&bar_sfree[sb]), ((j >> 1) - 1) & 1, &abort_flag, 4)) break;
+        if (j >= 2) go = go && px_wait(smem_u32(&bar_sfree[sb]), ((j >> 1) - 1) & 1, &abort_flag, 4);
         tc_fence_after();
         __syncwarp();
-        if (elect_one()) {
+        if (elect_one() && go) {
           const uint64_t k_desc = k_desc0 + uint64_t((stg * C::kStageBytes) >> 4), ksf_desc = ksf_desc0 + uint64_t((stg * C::kStageBytes) >> 4);
           const uint32_t sfk = tmem_base + C::kColSfk + sb * 4 * C::kMma;
 #pragma unroll
