@@ -317,6 +317,8 @@ int64_t ri_resattn_counter_bytes(int batch, int num_q_heads);
  *   prefix_splits   pieces of the prefix (the grid of the first launch: pieces x KV heads x 128-row tiles); 0 = no such
  *                   launch, every sequence reads all its tokens
  *   splits          pieces of the tokens behind the prefix, per sequence
+ *   max_kv_len      the length that these pieces divide evenly, usually an upper bound of seq_lens (0: a whole table row);
+ *                   the last piece takes what a longer sequence has beyond it
  *   workspace       ri_resattn_shared_prefix_workspace_bytes() bytes, 32-byte aligned, contents of no matter, owned by this
  *                   call until it has run: partials (o, l, m) of all pieces, and tickets
  *   out             bf16 or fp32 [B, Hq, D]; score_scale > 0 */

@@ -112,7 +112,8 @@ __global__ void __launch_bounds__(TlCfg<D>::kThreads, D == 128 ? 4 : 2) resattn_
     x1 = __ldcg(src + 1);
   }
   const int L = min(max(__ldcg(p.seq_lens + b), 0), p.max_tokens);
-  const int end = L > p.kv_begin ? min(begin + p.groups_per_split, (L + 15) / 16) : begin;
+  // the last piece goes to the sequence's end: one longer than the caller's bound costs time, not tokens
+  const int end = L > p.kv_begin ? (split == p.splits - 1 ? max(begin, (L + 15) / 16) : min(begin + p.groups_per_split, (L + 15) / 16)) : begin;
   const int i8 = lane >> 2, q4 = lane & 3;
   float o[C::kMTiles][4];
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};              // heads 2 q4, 2 q4 + 1

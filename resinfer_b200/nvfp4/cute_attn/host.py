@@ -303,9 +303,10 @@ def run_paged_fp4_decode_shared_prefix(q: torch.Tensor, pool: NvFp4PagedKVPool, 
 
     ``block_tables`` and ``seq_lens`` are the decode's own: whole sequences, prefix included; row ``prefix_row`` must hold
     all pages of the prefix, written as far as the longest sequence goes (rows may be padding, of length 0, or end inside the
-    prefix).  ``sm_scale`` includes the K global scale, ``value_scale`` is the V global scale.  ``max_seq_len``: an upper bound of ``seq_lens`` (0: taken from the
-    device, which synchronises).  ``plan``: (pieces of the prefix, pieces of the rest), chosen here without it.  BF16
-    output; V and P in FP16."""
+    prefix).  ``sm_scale`` includes the K global scale, ``value_scale`` is the V global scale.  ``max_seq_len``: an upper bound
+    of ``seq_lens`` (0: taken from the device, which synchronises); sequences that have outgrown it, in a captured graph say,
+    take longer and lose nothing.  ``plan``: (pieces of the prefix, pieces of the rest), chosen here without it.  BF16 output;
+    V and P in FP16."""
     _check_pool(pool)
     b, hq, d = q.shape
     check_shape_supported(hq, pool.num_kv_heads, d, prediction=1)
