@@ -345,8 +345,8 @@ extern "C" int ri_kv_read_nvfp4(const uint8_t* k_data, const uint8_t* k_sf, cons
   cudaLaunchConfig_t cfg{};
   const int units = num_kv_heads * (head_dim / 16);
   // Four tokens a thread where that leaves several waves of CTAs; one below.  us for one / four at 8 heads of 128: from slots
-  // 2048 tokens 3.6 / 5.2, 65536 57.2 / 55.1, 131072 111.0 / 106.6; from a block table 24576 tokens 23.5 / 24.2, 131072
-  // 112.7 / 109.8; 40001 tokens in 48 sequences, 4 heads of 256, 41.7 / 39.9.
+  // 2048 tokens 3.6 / 5.2, 65536 57.2 / 55.1, 131072 111.0 / 106.6; from a block table 24576 tokens 23.5 / 24.2, 65536
+  // 57.7 / 57.6, 131072 112.7 / 109.8; 40001 tokens in 48 sequences, 4 heads of 256, 41.7 / 39.9.
   const bool wide = num_tokens * units >= int64_t(di.sm_count) * 2048 * 8;
   geometry(num_tokens, units, wide ? 4 : 1, &cfg);
   cfg.stream = static_cast<cudaStream_t>(stream);

@@ -21,13 +21,14 @@
 // 512 + 256 for the two products -- and, close behind, issue slots and the latencies of the chain scores -> P -> product.
 // So the two softmax groups run free of each other: a group takes a step's exponentials with the maximum that it knows,
 // raised where the step itself shows a row grown beyond 2^8 times it; what the other group raised meanwhile is seen once the
-// products of the step in front are complete, and P is then scaled by the difference -- exactly, maxima being whole powers
-// of two.  (Waiting for the other group's maximum first, or taking turns at the exponentials, cost more than it hid; so did a
+// products of the step in front are complete, and P is then scaled by the difference -- exactly down to FP16's smallest
+// normal number, maxima being whole powers of two; below it a P of at most 2^-14 loses last bits.  (Waiting for the other group's maximum first, or taking turns at the exponentials, cost more than it hid; so did a
 // polynomial in the place of an eighth, a quarter or half of the exponentials: 128 steps 121, 139, 146 us against 119.)
-// Measured: a step of 128 x 128 (head_dim 256: 128 x 64) 0.78 us with pages of 128 tokens, 1480 cycles, the special function
-// unit busy for 60 % and the tensor cores for 44 to 51 %; 0.87 us with pages of 16.  Before the first step 4 us (the query's
-// codes 2), behind the last 3.  64 sequences of 64 heads over 8 behind 32768 tokens, in four pieces on 128 SMs: 57 us, 1.2
-// PFLOP/s of the two products.
+// Measured (differences of two lengths, back to back, 1.93 GHz): a step of 128 x 128 0.90 us with pages of 128 tokens, 1730
+// cycles, the special function unit busy for 59 % and the tensor cores for 43 to 50 %; 0.92 us with pages of 32, 0.96 with
+// pages of 16; head_dim 256 (128 x 64) 0.90.  Before the first step 4 us (the query's codes 2), behind the last 3.  64
+// sequences of 64 heads over 8 behind 32768 tokens and no further ones, in four pieces on 128 SMs: 70 us with the launch that
+// merges, 0.99 PFLOP/s of the two products.
 //
 // Roles (16 warps):
 //   0-3, 4-7   softmax, thread = row (tensor-memory lane); the first group takes the even steps, the second the odd ones
@@ -35,7 +36,7 @@
 //   12, 13     one thread each issues the scores' and the P.V products; warp 12 lays K's scales out for them
 //   14, 15     copies of codes (tiled TMA in the operand swizzle) and of scales (bulk), one lane per run of tokens that lie
 //              together in a page.  Small copies are what pages of 16 and 32 tokens cost: with V among them, all from one warp, a
-//              step took 1.8 us, from two warps 1.17; there the conversion warps load V themselves (0.87).
+//              step took 1.8 us, from two warps 1.17; there the conversion warps load V themselves (0.96).
 // Every wait is bounded.  A role whose wait expires sets the abort flag and leaves its loop (the scores': issues nothing more),
 // the others follow at their next wait that is not over, and none begins a copy or a product after that.  What is in flight
 // then is waited for whatever the flag says (px_drain): the products by a commit of their own, the copies by the barriers
