@@ -308,8 +308,8 @@ int64_t ri_resattn_counter_bytes(int batch, int num_q_heads);
  * up to roundings: the query is NVFP4(q) + NVFP4(q - NVFP4(q)) with exact differences, where ri_resattn_decode* take them
  * with an approximate reciprocal and settle differences that lie between two codes another way (2e-3 of the output).
  * Tokens of the prefix that no sequence reaches need not have been written.
- * A NaN in the query counts as in the quantisers: not for its block's magnitude, 16 of them as zeros.  NaN block scales of K
- * give NaN in the rows of their KV head that attend to them; those of V inside the prefix also in rows that end before them.
+ * A NaN in the query counts as in the quantisers: not for its block's magnitude, 16 of them as zeros.  NaN block scales in
+ * the cache (ri_kv_write_nvfp4 writes none) give NaN in the rows that attend to them: K's in all columns, V's in the block's.
  *   block_tables [batch, bt_stride] (bt_cols valid columns) cover every sequence from its first token; prefix_table is a
  *   row that holds the prefix's pages (usually block_tables itself, its first row).  A sequence no longer than the prefix
  *   attends to its own seq_lens[b] tokens of it; an empty one gives zeros.  The prefix may end inside a page (sequences

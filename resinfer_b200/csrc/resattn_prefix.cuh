@@ -222,6 +222,7 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
   __shared__ volatile int abort_flag;
   __shared__ volatile int copied[2];                           // steps whose codes (scales) have been asked for
   __shared__ float row_m[C::kRows], row_l[C::kRows];           // running maxima; row sums of the second group
+  __shared__ int nan_from[C::kSfPerRow];                       // the first token whose V has a NaN scale in a block, INT_MAX without one
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.x, hkv = blockIdx.y % p.hkv, row0 = (blockIdx.y / p.hkv) * C::kRows;
@@ -263,6 +264,8 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
       mbar_init(smem_u32(&bar_end[s]), 1);
     }
     abort_flag = 0;
+#pragma unroll
+    for (int i = 0; i < C::kSfPerRow; ++i) nan_from[i] = 0x7fffffff;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == C::kQkWarp) {
@@ -473,6 +476,9 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
           float o[16];
           tmem_ld16(lane_base + C::kColO + c, o);
           if (row < rows) {
+            if (lim > nan_from[c / 16])
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __int_as_float(0x7fffffff);
             float* dst = p.o_part + slot * D + c;              // 32-byte aligned: whole sectors
 #pragma unroll
             for (int i = 0; i < 16; i += 8)
@@ -531,6 +537,19 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
         nsf = __ldg(reinterpret_cast<const uint2*>(scales_at(row)));
       }
     };
+    // A NaN scale would reach every row of the tile, 0 x NaN, also those that end before its token: the block is taken as zeros,
+    // and the rows that attend to it get their NaN at the end.  (Where it is looked for, and how much code that adds to the
+    // loop, matters by 2 to 4 %: in front of the wait for the operand's buffer, and short, with scales that are in registers
+    // already, behind it and unrolled with those from the stages.  So placed it costs nothing to 0.8 %.)
+    constexpr int kNanUnroll = VDIRECT ? 1 : 4;
+    auto has_nan = [](uint32_t scales) { return (((scales & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0; };
+    auto take_out_nans = [&](uint32_t& scales, int j, int dblk) {
+      const uint32_t nans = ((scales & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+#pragma unroll kNanUnroll
+      for (int i = 0; i < 4; ++i)
+        if (nans >> (8 * i + 7) & 1) atomicMin(&nan_from[dblk * 4 + i], (s_begin + j) * kStep + tok);
+      scales &= ~((nans >> 7) * 0xFFu);
+    };
     if constexpr (VDIRECT) {
       const int first = page_of(0);
 #pragma unroll
@@ -573,10 +592,18 @@ __global__ void __launch_bounds__(PxCfg<D>::kThreads, 1) resattn_prefix_kernel(c
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar_empty[stg])); // the codes are in registers: the stage may be refilled
       }
+      if constexpr (VDIRECT) {
+        if (has_nan(sfw[0]) | has_nan(sfw[1])) {
+          take_out_nans(sfw[0], j, dblk0);
+          take_out_nans(sfw[1], j, dblk0 + 1);
+        }
+      }
       if (j >= 2 && !px_wait_warp(smem_u32(&bar_vfree[vb]), ((j >> 1) - 1) & 1, &abort_flag, 11)) break;
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         const int dblk = dblk0 + u;
+        if constexpr (!VDIRECT)
+          if (has_nan(sfw[u])) take_out_nans(sfw[u], j, dblk);
         const uint32_t words[8] = {c0[u].x, c0[u].y, c0[u].z, c0[u].w, c1[u].x, c1[u].y, c1[u].z, c1[u].w};
         uint32_t lo, hi, sc2[4];                               // the four block scales as FP16 pairs (s, s)
         asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
