@@ -24,10 +24,10 @@
 // products of the step in front are complete, and P is then scaled by the difference -- exactly down to FP16's smallest
 // normal number, maxima being whole powers of two; below it a P of at most 2^-14 loses last bits.  (Waiting for the other group's maximum first, or taking turns at the exponentials, cost more than it hid; so did a
 // polynomial in the place of an eighth, a quarter or half of the exponentials: 128 steps 121, 139, 146 us against 119.)
-// Measured (differences of two lengths, back to back, 1.93 GHz): a step of 128 x 128 0.90 us with pages of 128 tokens, 1730
-// cycles, the special function unit busy for 59 % and the tensor cores for 43 to 50 %; 0.92 us with pages of 32, 0.96 with
-// pages of 16; head_dim 256 (128 x 64) 0.90.  Before the first step 4 us (the query's codes 2), behind the last 3.  64
-// sequences of 64 heads over 8 behind 32768 tokens and no further ones, in four pieces on 128 SMs: 70 us with the launch that
+// Measured (differences of two lengths, back to back, 1.93 GHz): a step of 128 x 128 0.89 us with pages of 128 tokens, 1720
+// cycles, the special function unit busy for 59 % and the tensor cores for 43 to 50 %; 0.93 us with pages of 32, 0.96 with
+// pages of 16; head_dim 256 (128 x 64) 0.86.  Before the first step 4 us (the query's codes 2), behind the last 3.  64
+// sequences of 64 heads over 8 behind 32768 tokens and no further ones, in four pieces on 128 SMs: 69 us with the launch that
 // merges, 0.99 PFLOP/s of the two products.
 //
 // Roles (16 warps):
